@@ -284,6 +284,76 @@ int std_collect_relevance(const void* q, const void* k_cache, const int32_t* vis
                           int Hkv, int D, int cap, float* rel_out, long long rel_stride, void* workspace,
                           size_t workspace_bytes, void* stream);
 
+/* ---- (g) paged K/V cache ----------------------------------------------- */
+
+/* A layer's K (or V) pool is [num_pages, Hkv, page_size, D], bf16 or (is_fp16)
+ * fp16, D 64 or 128, page_size 16, 32, 64, 128 or 256.  Request b's token at
+ * position x lies in page block_table[b][x / page_size] (block_table [B,
+ * max_blocks] int32), row x % page_size; its slot is page * page_size + row.
+ * B <= STD_PAGED_MAX_REQUESTS; num_pages * page_size, max_blocks * page_size
+ * and B * max_blocks fit int32.  No reference counterpart (the reference's
+ * caches are contiguous). */
+#define STD_PAGED_MAX_REQUESTS 8192
+
+/* One step's tables, from the requests' lengths (all arrays on the device).
+ * Request b has past_lens[b] tokens cached and brings new_lens[b] >= 0; after
+ * the call it holds exactly the ceil((past + new) / page_size) pages that
+ * these need (n_blocks [B], its first entries of block_table).  Pages beyond
+ * come off its row (entries become -1) and go on the free list free_pages
+ * [num_pages], whose first *n_free entries are the free ones; missing pages
+ * come from the list's end, in request order.  new_lens 0 with a smaller
+ * past_lens thus rolls a request back, past_lens 0 releases it, and a return
+ * right after the take that it undoes restores tables and list exactly.
+ * A request whose needed pages, with those of the requests before it, are more
+ * than the list holds (after this call's returns) is refused: admitted[b] 0,
+ * kv_lens[b] 0, its pages as before.  The others: admitted[b] 1, kv_lens[b] =
+ * past + new.  cu_q [B + 1]: exclusive sums of new_lens, refused ones
+ * included.  slots, positions [max_tokens]: where token i of the step (request
+ * order) goes; -1 for tokens of refused requests and past the last token.
+ * max_tokens 0: neither is written (they may be NULL).
+ * A negative length, one beyond max_blocks * page_size or an n_blocks outside
+ * [0, max_blocks] refuses the request and is reported (device error 3), as are
+ * more than max_tokens tokens unless max_tokens is 0 (the rest have no slot);
+ * a page id or list length outside the pool is reported (error 2), the id gives
+ * slot -1.  Inputs and outputs must not overlap. */
+int std_paged_update(const int32_t* past_lens, const int32_t* new_lens, int32_t* block_table, int32_t* n_blocks,
+                     int32_t* free_pages, int32_t* n_free, int B, int max_blocks, int page_size, int num_pages,
+                     int max_tokens, int32_t* cu_q, int32_t* kv_lens, int32_t* slots, int32_t* positions,
+                     int32_t* admitted, void* stream);
+
+/* RoPE and append by slot: rows of qkv [T, (Hq+2Hkv)*D]; q and k rotated at
+ * positions[t] with cos/sin tables [max_pos, D/2] of the same type (fp32
+ * arithmetic, rounded once), q to q_out [T, Hq, D], k and v to slots[t] of the
+ * pools.  positions[t] < 0: row t is skipped, q_out's row left as it was;
+ * slots[t] < 0: k and v are not stored.  A position >= max_pos is reported and
+ * read as max_pos - 1, a slot outside the pool is reported and not stored
+ * (error 2).  Slots of a call must differ. */
+int std_paged_rope_append(const void* qkv, int T, int Hq, int Hkv, int D, int is_fp16, const int32_t* positions,
+                          const int32_t* slots, const void* cos_t, const void* sin_t, int max_pos, void* q_out,
+                          void* k_pages, void* v_pages, int num_pages, int page_size, void* stream);
+
+/* Attention of the new tokens over the paged cache: the paged, ragged form of
+ * std_verify_attn (modeling_qwen2_5_vl.py:1096-1133) for chunks of any length.
+ * Request b's n = cu_q[b+1] - cu_q[b] tokens are rows cu_q[b].. of q [T, Hq,
+ * D] (T >= cu_q[B]); their keys are in the cache.  It has kv_lens[b] keys, the
+ * n new ones last; causal: token t sees keys 0 .. kv_len - n + t, else all
+ * kv_len.  out [T, Hq, D]; lse [T, Hq] fp32 natural log (may be NULL).  A row
+ * that sees no key gives 0 and -inf; rows outside every request are left as
+ * they were.  scale > 0; Hq / Hkv a whole number <= 128.  What lies in the
+ * cache past a request's keys is not used, whatever it holds; a non-finite V
+ * row of a new token may reach the other new tokens of its request.
+ * A cu_q or kv_lens entry that does not fit T or max_blocks is reported (error
+ * 3), the request skipped or its keys cut; a page id outside the pool is
+ * reported (error 2) and read as zeros.
+ * Same inputs, same bits; a request's last bits may depend on the batch it is
+ * in (std_verify_attn's do not).  The workspace
+ * (std_paged_attn_workspace_bytes) is that of one call at a time. */
+size_t std_paged_attn_workspace_bytes(int D);
+int std_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int32_t* block_table,
+                   const int32_t* cu_q, const int32_t* kv_lens, int T, int B, int Hq, int Hkv, int D, int is_fp16,
+                   int num_pages, int page_size, int max_blocks, int causal, float scale, void* out, float* lse,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- GEMM tuning and plan --------------------------------------------- */
 
 /* Tuning (no reference counterpart): the per-CTA shared-memory budget of the

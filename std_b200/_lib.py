@@ -83,6 +83,10 @@ SIGNATURES: Dict[str, tuple] = {
     "std_capture_while_begin": (I, [P, P, PI32, I, PI32, P, P]),
     "std_capture_while_end": (I, [P, ctypes.c_ulonglong, PI32, I, PI32, I]),
     "std_launch_count": (I64, []),
+    "std_paged_update": (I, [PI32, PI32, PI32, PI32, PI32, PI32, I, I, I, I, I, PI32, PI32, PI32, PI32, PI32, P]),
+    "std_paged_rope_append": (I, [P, I, I, I, I, I, PI32, PI32, P, P, I, P, P, P, I, I, P]),
+    "std_paged_attn_workspace_bytes": (SZ, [I]),
+    "std_paged_attn": (I, [P, P, P, PI32, PI32, PI32, I, I, I, I, I, I, I, I, I, I, F, P, PF, P, SZ, P]),
 }
 
 _STATUS = {1: "bad shape or argument", 2: "capacity exceeded", 3: "unsupported device or driver entry point",

@@ -5,6 +5,7 @@
 // device code.  Build: std_b200/build.py (nvcc -gencode
 // arch=compute_100a,code=sm_100a -shared).
 #include "common.cuh"
+#include "std_b200.h"
 
 #include "decode_ops.cu"
 #include "draft_attn.cu"
@@ -15,6 +16,8 @@
 #include "gemm.cu"
 #include "graph_loop.cu"
 #include "collect.cu"
+#include "paged_ops.cu"
+#include "paged_attn.cu"
 
 extern "C" int std_version(void) { return 100; }
 

@@ -374,5 +374,157 @@ def argmax_rows(logits: torch.Tensor, out: torch.Tensor, n: int = 1, out_stride:
     return out
 
 
+# ----------------------------------------------------------------------------
+# paged K/V cache
+# ----------------------------------------------------------------------------
+
+_PAGED_DTYPES = (torch.bfloat16, torch.float16)
+
+
+def _paged_tensor(t: torch.Tensor, name: str, shape: Tuple[int, ...], dtype: torch.dtype, device: torch.device) -> None:
+    """A contiguous tensor of this shape and type on the call's device."""
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError(f"{name} must be a tensor")
+    _check(t, dtype, name)
+    if t.device != device:
+        raise RuntimeError(f"{name} is on {t.device}, the call's other tensors on {device}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {list(shape)}, got {list(t.shape)}")
+
+
+def _paged_device(t: torch.Tensor, name: str) -> torch.device:
+    """The call's device: kernels run on the current device's stream, so it
+    has to be that one."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor (no CPU path)")
+    if t.device.index != torch.cuda.current_device():
+        raise RuntimeError(f"{name} is on {t.device}, but cuda:{torch.cuda.current_device()} is the current device")
+    return t.device
+
+
+def _paged_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtype,
+                device: torch.device) -> Tuple[int, int, int, int]:
+    if k_pages.dim() != 4:
+        raise ValueError("k_pages must be [num_pages, Hkv, page_size, D]")
+    _paged_tensor(k_pages, "k_pages", k_pages.shape, dtype, device)
+    _paged_tensor(v_pages, "v_pages", k_pages.shape, dtype, device)
+    num_pages, Hkv, page, D = k_pages.shape
+    if page not in (16, 32, 64, 128, 256):
+        raise ValueError(f"page_size must be 16, 32, 64, 128 or 256, got {page}")
+    if D not in (64, 128):
+        raise ValueError(f"head dim must be 64 or 128, got {D}")
+    return num_pages, Hkv, page, D
+
+
+def paged_update(past_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, n_blocks: torch.Tensor,
+                 free_pages: torch.Tensor, n_free: torch.Tensor, page_size: int, max_tokens: int,
+                 out: Optional[Tuple[torch.Tensor, ...]] = None):
+    """One step's tables of a paged cache, from the requests' lengths.
+
+    past_lens, new_lens [B]; block_table [B, max_blocks], n_blocks [B],
+    free_pages [num_pages] and n_free [1] are updated in place (all int32 on the
+    device): every request ends up with the pages that past + new tokens need,
+    taken from or returned to the end of the free list, so new_lens 0 with a
+    shorter past_lens rolls a request back.  Returns (cu_q [B + 1], kv_lens [B],
+    slots [max_tokens], positions [max_tokens], admitted [B]); a request that the
+    list cannot serve has admitted 0, kv_lens 0 and slots -1.  `out` gives the
+    five result tensors (a captured graph's static buffers)."""
+    device = _paged_device(past_lens, "past_lens")
+    B, i32 = past_lens.numel(), torch.int32
+    if B < 1:
+        raise ValueError("paged_update needs at least one request")
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be [B, max_blocks]")
+    width, num_pages = block_table.shape[1], free_pages.numel()
+    if not 0 <= int(max_tokens) < 2 ** 31:
+        raise ValueError("max_tokens must be a non-negative int32")
+    for t, name, shape in ((past_lens, "past_lens", (B,)), (new_lens, "new_lens", (B,)),
+                           (block_table, "block_table", (B, width)), (n_blocks, "n_blocks", (B,)),
+                           (free_pages, "free_pages", (num_pages,)), (n_free, "n_free", (1,))):
+        _paged_tensor(t, name, shape, i32, device)
+    if out is None:
+        out = tuple(torch.empty(n, dtype=i32, device=device) for n in (B + 1, B, max_tokens, max_tokens, B))
+    cu_q, kv_lens, slots, positions, admitted = out
+    for t, name, n in ((cu_q, "cu_q", B + 1), (kv_lens, "kv_lens", B), (slots, "slots", max_tokens),
+                       (positions, "positions", max_tokens), (admitted, "admitted", B)):
+        _paged_tensor(t, name, (n,), i32, device)
+    _lib.call("std_paged_update", past_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
+              n_blocks.data_ptr(), free_pages.data_ptr(), n_free.data_ptr(), B, width, int(page_size), num_pages,
+              int(max_tokens), cu_q.data_ptr(), kv_lens.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+              admitted.data_ptr(), _stream())
+    return cu_q, kv_lens, slots, positions, admitted
+
+
+def paged_rope_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, cos_t: torch.Tensor,
+                      sin_t: torch.Tensor, q_out: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor):
+    """RoPE of qkv [T, (Hq + 2 Hkv) * D]'s q and k at positions [T]; q goes to
+    q_out [T, Hq, D], k and v to slots [T] of the pools [num_pages, Hkv, page,
+    D].  Position -1: the row is skipped; slot -1: nothing is stored.  bf16 or
+    fp16 throughout (tables cos_t, sin_t [max_pos, D / 2] too)."""
+    device = _paged_device(qkv, "qkv")
+    dtype = qkv.dtype
+    if dtype not in _PAGED_DTYPES:
+        raise RuntimeError(f"qkv must be bfloat16 or float16, got {dtype}")
+    if q_out.dim() != 3 or cos_t.dim() != 2:
+        raise ValueError("q_out must be [T, Hq, D] and cos_t [max_pos, D / 2]")
+    num_pages, Hkv, page, D = _paged_pool(k_pages, v_pages, dtype, device)
+    T, Hq = q_out.shape[:2]
+    max_pos = cos_t.shape[0]
+    for t, name, shape in ((q_out, "q_out", (T, Hq, D)), (qkv, "qkv", (T, (Hq + 2 * Hkv) * D)),
+                           (cos_t, "cos_t", (max_pos, D // 2)), (sin_t, "sin_t", (max_pos, D // 2))):
+        _paged_tensor(t, name, shape, dtype, device)
+    for t, name in ((positions, "positions"), (slots, "slots")):
+        _paged_tensor(t, name, (T,), torch.int32, device)
+    _lib.call("std_paged_rope_append", qkv.data_ptr(), T, Hq, Hkv, D, 1 if dtype == torch.float16 else 0,
+              positions.data_ptr(), slots.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), max_pos, q_out.data_ptr(),
+              k_pages.data_ptr(), v_pages.data_ptr(), num_pages, page, _stream())
+    return q_out
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                    cu_q: torch.Tensor, kv_lens: torch.Tensor, causal: bool = True, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None):
+    """Attention of each request's new tokens over its paged cache.
+
+    q [T, Hq, D]: request b's tokens are rows cu_q[b] .. cu_q[b+1] - 1 (cu_q [B +
+    1] int32); pools [num_pages, Hkv, page, D]; block_table [B, max_blocks] and
+    kv_lens [B] int32, the new tokens' keys included.  Token t of n sees keys 0 ..
+    kv_len - n + t (causal) or all kv_len.  bf16 or fp16; any Hq / Hkv up to 128.
+    scale defaults to 1 / sqrt(D).  out [T, Hq, D], lse [T, Hq] fp32 (optional).
+    Rows that see no key give 0 and -inf; rows outside every request are left
+    as they were (uninitialised in an `out` made here)."""
+    device = _paged_device(q, "q")
+    dtype = q.dtype
+    if dtype not in _PAGED_DTYPES:
+        raise RuntimeError(f"q must be bfloat16 or float16, got {dtype}")
+    if q.dim() != 3 or block_table.dim() != 2:
+        raise ValueError("q must be [T, Hq, D] and block_table [B, max_blocks]")
+    T, Hq, D = q.shape
+    num_pages, Hkv, page, _ = _paged_pool(k_pages, v_pages, dtype, device)
+    B, width = block_table.shape
+    _paged_tensor(q, "q", (T, Hq, k_pages.shape[3]), dtype, device)
+    if Hkv < 1 or Hq % Hkv != 0 or not 1 <= Hq // Hkv <= 128:
+        raise ValueError(f"query heads ({Hq}) must be a multiple of key heads ({Hkv}), at most 128 times as many")
+    for t, name, shape in ((block_table, "block_table", (B, width)), (cu_q, "cu_q", (B + 1,)),
+                           (kv_lens, "kv_lens", (B,))):
+        _paged_tensor(t, name, shape, torch.int32, device)
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not 0.0 < scale < 3e38:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _paged_tensor(out, "out", (T, Hq, D), dtype, device)
+    if lse is not None:
+        _paged_tensor(lse, "lse", (T, Hq), torch.float32, device)
+    # Of this call alone: the caching allocator hands it out in stream order, and
+    # under capture from the graph's own pool, so no two calls or graphs share it.
+    ws = torch.empty(_lib.query("std_paged_attn_workspace_bytes", D), dtype=torch.uint8, device=device)
+    _lib.call("std_paged_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
+              cu_q.data_ptr(), kv_lens.data_ptr(), T, B, Hq, Hkv, D, 1 if dtype == torch.float16 else 0, num_pages,
+              page, width, 1 if causal else 0, scale, out.data_ptr(), _p(lse), ws.data_ptr(), ws.numel(), _stream())
+    return out
+
+
 def device_error() -> int:
     return _lib.device_error()

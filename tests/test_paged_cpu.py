@@ -1,0 +1,83 @@
+"""CPU: the paged-cache entry points refuse what they cannot serve, before any CUDA call."""
+import ctypes
+
+import pytest
+import torch
+
+from std_b200 import _lib, ops
+
+A = 1 << 20  # a 16-byte aligned address that is never read
+
+
+def attn(**kw):
+    a = dict(q=A, k=A, v=A, table=A, cu=A, lens=A, T=4, B=1, Hq=28, Hkv=4, D=128, fp16=0, pages=8, page=16, width=4,
+             causal=1, scale=0.1, out=2 * A, lse=None, ws=A, nb=1 << 40, stream=None)
+    assert not set(kw) - set(a)
+    a.update(kw)
+    return _lib.load().std_paged_attn(*a.values())
+
+
+@pytest.mark.parametrize("bad", [
+    dict(D=96), dict(D=0), dict(T=-1), dict(B=0), dict(B=8193), dict(Hkv=0), dict(Hq=30), dict(Hq=0), dict(Hq=129, Hkv=1),
+    dict(page=8), dict(page=48), dict(page=0), dict(pages=0), dict(width=0), dict(scale=0.0), dict(scale=-1.0),
+    dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(k=None), dict(v=None), dict(table=None),
+    dict(cu=None), dict(lens=None), dict(out=None), dict(out=A), dict(q=A + 8), dict(k=A + 2), dict(out=2 * A + 4),
+    dict(pages=1 << 27, page=16), dict(width=1 << 27, page=16), dict(pages=1 << 22, page=256, Hkv=28)])
+def test_attention_refusals(bad):
+    assert attn(**bad) == 1
+
+
+def test_attention_workspace_and_nothing_to_do():
+    need = _lib.query("std_paged_attn_workspace_bytes", 128)
+    assert need > 0 and _lib.query("std_paged_attn_workspace_bytes", 96) == 0
+    assert attn(nb=need - 1) == 5 and attn(ws=None) == 5 and attn(ws=A + 8) == 5
+    assert attn(T=0, q=None, out=None) == 0
+
+
+def update(**kw):
+    a = dict(past=A, new=A, table=A, nblk=A, free=A, nfree=A, B=2, width=4, page=16, pages=8, tokens=3, cu=A, kv=A,
+             slots=A, pos=A, ok=A, stream=None)
+    assert not set(kw) - set(a)
+    a.update(kw)
+    return _lib.load().std_paged_update(*a.values())
+
+
+@pytest.mark.parametrize("bad", [
+    dict(B=0), dict(B=8193), dict(width=0), dict(page=24), dict(pages=0), dict(tokens=-1), dict(past=None),
+    dict(new=None), dict(table=None), dict(nblk=None), dict(free=None), dict(nfree=None), dict(cu=None), dict(kv=None),
+    dict(slots=None), dict(pos=None), dict(ok=None), dict(B=8192, width=1 << 20), dict(pages=1 << 28),
+    dict(width=1 << 28, B=1)])
+def test_update_refusals(bad):
+    assert update(**bad) == 1
+
+
+def append(**kw):
+    a = dict(qkv=A, T=3, Hq=28, Hkv=4, D=128, fp16=0, pos=A, slots=A, cos=A, sin=A, max_pos=9, q=A, k=A, v=A, pages=8,
+             page=16, stream=None)
+    assert not set(kw) - set(a)
+    a.update(kw)
+    return _lib.load().std_paged_rope_append(*a.values())
+
+
+@pytest.mark.parametrize("bad", [
+    dict(T=-1), dict(Hq=0), dict(Hkv=0), dict(D=80), dict(max_pos=0), dict(pages=0), dict(page=20), dict(pages=1 << 28),
+    dict(qkv=None), dict(pos=None), dict(slots=None), dict(cos=None), dict(sin=None), dict(q=None), dict(k=None),
+    dict(v=None), dict(qkv=A + 2), dict(cos=A + 4), dict(q=A + 8), dict(k=A + 8)])
+def test_append_refusals(bad):
+    assert append(**bad) == 1
+
+
+def test_append_nothing_to_do():
+    assert append(T=0, qkv=None, q=None) == 0
+
+
+def test_wrappers_refuse_cpu_tensors():
+    i = torch.zeros(2, dtype=torch.int32)
+    k = torch.zeros(2, 1, 16, 64, dtype=torch.bfloat16)
+    q = torch.zeros(2, 1, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.paged_attention(q, k, k, i.view(1, 2), i, i[:1])
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.paged_update(i, i, i.view(2, 1), i, i, i[:1], 16, 4)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.paged_rope_append(q.view(2, 64), i, i, k[0, 0], k[0, 0], q, k, k)

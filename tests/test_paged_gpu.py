@@ -1,0 +1,360 @@
+"""GPU: the paged K/V cache operators (tables from lengths, append by slot,
+attention over pages) against plain 64-bit implementations.
+
+Tolerances.  e = finfo(dtype).eps; rounding to dtype is off by at most e / 2.
+Attention: an output is rounded once (e/2 |o|) and each probability once (e/2,
+so e/2 A with A = sum p |v| / sum p; half precision also loses up to 2^-25 of a
+probability below 2^-14, the largest being at least 1 in the kernel's units).
+Scores are 32-bit sums of D products: off by at most D 2^-24 sum |q k| scale each
+way, which with the exponential's own 2^-22 is a relative error d of each
+probability, in numerator and denominator: 2 d A.  Sums of n probabilities add
+at most (34 + n / 64) 2^-24.
+"""
+import math
+import random
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from std_b200 import ops as _ops
+
+    assert torch.cuda.is_available()
+    return _ops
+
+
+def _no_device_error(ops):
+    torch.cuda.synchronize()
+    assert ops.device_error() == 0
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+# ------------------------------------------------------------------ attention
+class Paged:
+    """Random queries and a shuffled paged cache of requests with (past, new)
+    lengths; everything no query may read is NaN."""
+
+    def __init__(self, pairs, Hq, Hkv, D, page, dtype, seed=0, tail_rows=0, kv=None, spare=3, scale_q=1.5):
+        g = torch.Generator().manual_seed(seed)
+        rng = random.Random(seed)
+        self.pairs, self.page, self.dtype = pairs, page, dtype
+        self.kv = [p + n for p, n in pairs] if kv is None else kv
+        blocks = [-(-k // page) for k in self.kv]
+        num_pages = sum(blocks) + spare
+        ids = list(range(num_pages))
+        rng.shuffle(ids)
+        width = max(blocks + [1]) + 2
+        table = torch.full((len(pairs), width), -1, dtype=torch.int32)
+        k = torch.full((num_pages, Hkv, page, D), float("nan"))
+        v = torch.full((num_pages, Hkv, page, D), float("nan"))
+        self.keys, at = [], 0
+        for b, nb in enumerate(blocks):
+            mine = ids[at:at + nb]
+            at += nb
+            table[b, :nb] = torch.tensor(mine, dtype=torch.int32)
+            L = self.kv[b]
+            kb = torch.randn(L, Hkv, D, generator=g).to(dtype)
+            vb = torch.randn(L, Hkv, D, generator=g).to(dtype)
+            self.keys.append((kb.cuda(), vb.cuda()))
+            for i, pg in enumerate(mine):
+                rows = slice(i * page, min(L, (i + 1) * page))
+                k[pg, :, :rows.stop - rows.start] = kb[rows].permute(1, 0, 2).float()
+                v[pg, :, :rows.stop - rows.start] = vb[rows].permute(1, 0, 2).float()
+        T = sum(n for _, n in pairs)
+        self.q = (torch.randn(T + tail_rows, Hq, D, generator=g) * scale_q).to(dtype).cuda()
+        self.k, self.v, self.table = k.to(dtype).cuda(), v.to(dtype).cuda(), table.cuda()
+        cu = [0]
+        for _, n in pairs:
+            cu.append(cu[-1] + n)
+        self.cu, self.kv_lens = _i32(cu), _i32(self.kv)
+
+    def call(self, ops, causal=True, **kw):
+        return ops.paged_attention(self.q, self.k, self.v, self.table, self.cu, self.kv_lens, causal=causal, **kw)
+
+    def check(self, out, lse, causal=True, scale=None):
+        Hq, D = self.q.shape[1:]
+        scale = 1 / math.sqrt(D) if scale is None else scale
+        e, at = torch.finfo(self.dtype).eps, 0
+        for b, (_, n) in enumerate(self.pairs):
+            L = self.kv[b]
+            if n == 0:
+                continue
+            q = self.q[at:at + n].double().permute(1, 0, 2)                    # [Hq, n, D]
+            G = Hq // self.k.shape[1]
+            k = self.keys[b][0].double().permute(1, 0, 2).repeat_interleave(G, 0)
+            v = self.keys[b][1].double().permute(1, 0, 2).repeat_interleave(G, 0)
+            s = q @ k.transpose(1, 2) * scale
+            size = (q.abs() @ k.abs().transpose(1, 2) * scale).amax(-1, keepdim=True) if L else s.new_zeros(Hq, n, 1)
+            if causal:
+                see = torch.arange(L, device="cuda")[None] <= (L - n + torch.arange(n, device="cuda"))[:, None]
+                s = s.masked_fill(~see, -math.inf)
+            m = s.amax(-1, keepdim=True) if L else s.new_full((Hq, n, 1), -math.inf)
+            some = m > -math.inf
+            p = torch.exp(s - torch.where(some, m, 0.0))
+            l = p.sum(-1, keepdim=True)
+            l1 = torch.where(some, l, 1.0)
+            ref, A = p @ v / l1, p @ v.abs() / l1
+            d = D * 2.0 ** -24 * size + 2.0 ** -22 + (34 + L / 64) * 2.0 ** -24
+            tol = 1.01 * (e / 2 * ref.abs() + (e / 2 + 2 * d) * A)
+            if self.dtype == torch.float16:
+                tol = tol + 2.0 ** -25 * (see.double() if causal else torch.ones_like(s)) @ v.abs() / l1 + 2.0 ** -25
+            got = out[at:at + n].double().permute(1, 0, 2)
+            off = (got - ref).abs()
+            assert torch.isfinite(got).all(), f"request {b}: non-finite output"
+            assert (off <= tol + 1e-30).all(), f"request {b} (L {L}, n {n}): off by {(off - tol).max().item():.3e} over"
+            if lse is not None:
+                want = torch.where(some, torch.where(some, m, 0.0) + l1.log(), -math.inf)[..., 0]
+                g2 = lse[at:at + n].double().t()
+                assert torch.equal(g2 == -math.inf, want == -math.inf)
+                fin = want > -math.inf
+                t2 = 2 * d[..., 0] + (want.abs() + m[..., 0].abs() + 16) * 2.0 ** -22
+                assert ((g2 - want).abs()[fin] <= t2[fin]).all()
+            at += n
+
+
+BF, FP = torch.bfloat16, torch.float16
+CASES = [
+    # pairs (past, new), Hq, Hkv, D, page, dtype, causal
+    ([(0, 1)], 28, 4, 128, 16, BF, True),
+    ([(199, 1)], 28, 4, 128, 16, BF, True),
+    ([(126, 1), (127, 1), (128, 1), (255, 1), (256, 1)], 28, 4, 128, 64, BF, True),
+    ([(300, 10), (1, 10), (1000, 18), (0, 18)], 28, 4, 128, 32, BF, True),
+    ([(50, 19), (77, 36), (130, 37), (5, 73)], 7, 1, 128, 128, BF, True),
+    ([(0, 0), (40, 3), (0, 0), (513, 0), (7, 1)], 28, 4, 128, 16, BF, True),
+    ([(0, 500)], 28, 4, 128, 64, BF, True),
+    ([(333, 301), (0, 129), (64, 1)], 16, 16, 64, 32, FP, True),
+    ([(333, 301), (0, 129), (64, 1)], 16, 16, 64, 256, BF, False),
+    ([(2000, 200), (90, 7)], 32, 8, 128, 256, FP, False),
+    ([(700, 5), (3, 4)], 128, 1, 64, 16, BF, True),
+    ([(700, 3), (3, 4), (1, 1)], 96, 2, 128, 32, FP, True),
+    ([(3999, 1)], 28, 4, 128, 64, BF, True),
+    ([(9000, 1), (20, 1)], 8, 1, 128, 16, BF, True),
+    ([(6000, 40)], 12, 2, 128, 64, BF, True),
+    ([(5, 1300)], 40, 8, 64, 16, FP, True),
+]
+
+
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_attention_against_64_bits(ops, case):
+    pairs, Hq, Hkv, D, page, dtype, causal = CASES[case]
+    x = Paged(pairs, Hq, Hkv, D, page, dtype, seed=case, tail_rows=3)
+    T = x.q.shape[0]
+    out = torch.full_like(x.q, 7.0)
+    lse = torch.full((T, Hq), 7.0, device="cuda")
+    got = x.call(ops, causal, out=out, lse=lse)
+    assert got is out
+    x.check(out, lse, causal)
+    # rows behind the last request are left as they were
+    assert (out[T - 3:] == 7).all() and (lse[T - 3:] == 7).all()
+    # same inputs, same bits, with and without the log-sum-exp
+    assert torch.equal(x.call(ops, causal)[:T - 3], out[:T - 3])
+    _no_device_error(ops)
+
+
+@pytest.mark.parametrize("B", [383, 385, 1000])
+def test_attention_many_requests(ops, B):
+    rng = random.Random(B)
+    pairs = [(rng.randint(0, 60), rng.choice([0, 1, 1, 2, 20])) for _ in range(B)]
+    x = Paged(pairs, 7, 1, 128, 16, BF, seed=B)
+    x.check(x.call(ops), None)
+    _no_device_error(ops)
+
+
+def test_rows_without_keys(ops):
+    """No keys at all, and fewer keys than new tokens: such rows give 0 and -inf."""
+    x = Paged([(0, 4), (0, 20), (0, 40), (10, 2)], 28, 4, 128, 16, BF, kv=[0, 13, 1, 12])
+    lse = torch.zeros(x.q.shape[:2], device="cuda")
+    out = x.call(ops, lse=lse)
+    x.check(out, lse)
+    assert (out[:4] == 0).all() and (lse[:4] == -math.inf).all()
+    x.check(x.call(ops, causal=False), None, causal=False)
+    _no_device_error(ops)
+
+
+def test_large_scores_and_scale(ops):
+    """Running maxima that jump (the accumulators are rescaled) and a user's scale."""
+    for scale_q, scale in ((40.0, None), (3.0, 0.7), (1.0, 1e-3)):
+        x = Paged([(1500, 30), (800, 1), (0, 300)], 28, 4, 128, 16, BF, seed=3, scale_q=scale_q)
+        x.check(x.call(ops, scale=scale), None, scale=scale)
+    _no_device_error(ops)
+
+
+# ------------------------------------------------------------------ tables
+def plain_update(past, new, table, n_blocks, free, n_free, page):
+    """The rules of paged_update, one page at a time; changes table, n_blocks,
+    free (a list) and returns the results and the new list length."""
+    B, width = len(past), len(table[0])
+    bad = [p < 0 or n < 0 or p + n > width * page or not 0 <= h <= width for p, n, h in zip(past, new, n_blocks)]
+    want = [h if x else -(-(p + n) // page) for p, n, h, x in zip(past, new, n_blocks, bad)]
+    back = [(b, j) for b in range(B) for j in range(want[b], n_blocks[b])]
+    stack = free[:n_free] + [table[b][j] for b, j in reversed(back)]
+    for b, j in back:
+        table[b][j] = -1
+    pool, ok, full = len(stack), [], False
+    free[:pool] = stack
+    for b in range(B):
+        need = max(0, want[b] - n_blocks[b])
+        full = full or need > pool
+        ok.append(not bad[b] and (need == 0 or not full))
+        if ok[b]:
+            for j in range(n_blocks[b], want[b]):
+                pool -= 1
+                table[b][j] = free[pool]
+            n_blocks[b] = want[b]
+    cu, slots, positions = [0], [], []
+    for b in range(B):
+        for x in range(past[b], past[b] + new[b]) if ok[b] else [None] * max(0, new[b]):
+            positions.append(-1 if x is None else x)
+            slots.append(-1 if x is None else table[b][x // page] * page + x % page)
+        cu.append(cu[-1] + max(0, new[b]))
+    kv = [p + n if o else 0 for p, n, o in zip(past, new, ok)]
+    return cu, kv, slots, positions, [int(o) for o in ok], pool
+
+
+class Tables:
+    """The state on the device and beside it in lists."""
+
+    def __init__(self, B, width, num_pages, page, seed):
+        self.rng = random.Random(seed)
+        ids = list(range(num_pages))
+        self.rng.shuffle(ids)
+        self.page, self.free, self.n_free = page, ids, num_pages
+        self.table, self.n_blocks = [[-1] * width for _ in range(B)], [0] * B
+        self.dev = [_i32(self.table), _i32(self.n_blocks), _i32(self.free), _i32([self.n_free])]
+
+    def step(self, ops, past, new, max_tokens, stream_out=None):
+        got = ops.paged_update(_i32(past), _i32(new), *self.dev, self.page, max_tokens, out=stream_out)
+        cu, kv, slots, pos, ok, self.n_free = plain_update(past, new, self.table, self.n_blocks, self.free, self.n_free,
+                                                           self.page)
+        slots, pos = (slots + [-1] * max_tokens)[:max_tokens], (pos + [-1] * max_tokens)[:max_tokens]
+        for g, w, name in zip(got, (cu, kv, slots, pos, ok), ("cu_q", "kv_lens", "slots", "positions", "admitted")):
+            assert g.tolist() == w, name
+        for g, w, name in zip(self.dev, (self.table, self.n_blocks, None, [self.n_free]),
+                              ("block_table", "n_blocks", "", "n_free")):
+            assert w is None or g.tolist() == w, name
+        assert self.dev[2].tolist()[:self.n_free] == self.free[:self.n_free], "free_pages"
+        return kv, ok
+
+
+@pytest.mark.parametrize("B,width,pages,page,most", [(1, 4, 5, 16, 20), (8, 40, 200, 64, 30), (33, 12, 150, 32, 60),
+                                                     (300, 20, 2500, 16, 40), (1500, 9, 4000, 128, 200)])
+def test_update_random_steps(ops, B, width, pages, page, most):
+    """A serving loop's steps: growth, rollback, release, refusals for lack of pages."""
+    x = Tables(B, width, pages, page, seed=B)
+    lens = [0] * B
+    for step in range(6):
+        new = [0 if x.rng.random() < 0.2 else x.rng.randint(0, most) for _ in range(B)]
+        past = [min(p, width * page - n) if x.rng.random() < 0.9 else 0 for p, n in zip(lens, new)]
+        total = sum(new)
+        kv, ok = x.step(ops, past, new, max(0, total + x.rng.choice([0, 0, 5])))
+        lens = [k if o else p for k, o, p in zip(kv, ok, past)]
+        if step % 2:  # some of the new tokens are given up again
+            lens = [max(0, p - x.rng.randint(0, most)) for p in lens]
+            kv, ok = x.step(ops, lens, [0] * B, 0)
+    _no_device_error(ops)
+
+
+def test_update_take_then_return_restores_everything(ops):
+    x = Tables(20, 30, 400, 16, seed=5)
+    past = [x.rng.randint(0, 200) for _ in range(20)]
+    x.step(ops, past, [0] * 20, 0)
+    before = [t.clone() for t in x.dev]
+    x.step(ops, past, [x.rng.randint(0, 100) for _ in range(20)], 2000)
+    x.step(ops, past, [0] * 20, 0)
+    for a, b in zip(before, x.dev):
+        assert torch.equal(a, b)
+
+
+def test_update_many_tokens(ops):
+    """More tokens than one block's threads, odd counts, one request holding most."""
+    x = Tables(9, 700, 3000, 16, seed=6)
+    x.step(ops, [0, 100, 7, 0, 3, 0, 0, 1, 2], [9001, 1, 0, 0, 130, 77, 16, 15, 17], 9300)
+    x.step(ops, [9001, 101, 7, 0, 133, 77, 16, 16, 19], [1200] + [600] * 8, 1200 + 600 * 8)
+    _no_device_error(ops)
+
+
+def test_update_reports_bad_lengths(ops):
+    """A negative length or one past the table refuses that request alone; too
+    many tokens and bad page ids are reported and nothing is written past the
+    outputs."""
+    x = Tables(4, 4, 30, 16, seed=7)
+    x.step(ops, [0, -5, 60, 3], [10, 4, 10, 2], 40)
+    assert ops.device_error() == 3
+    x.step(ops, [10, 0, 0, 5], [3, 0, 2, -1], 40)
+    assert ops.device_error() == 3
+    outs = [torch.full((n,), 99, dtype=torch.int32, device="cuda") for n in (5, 4, 8, 8, 4)]
+    guard = torch.full((3, 8), 99, dtype=torch.int32, device="cuda")
+    ops.paged_update(_i32([13, 0, 2, 5]), _i32([20, 0, 0, 0]), *x.dev, 16, 8, out=(outs[0], outs[1], guard[0], guard[1], outs[4]))
+    assert (guard[2] == 99).all() and guard[1].tolist() == list(range(13, 21))
+    assert ops.device_error() == 3
+    table = _i32([[1000, -1]])
+    got = ops.paged_update(_i32([4]), _i32([2]), table, _i32([1]), _i32([0, 1]), _i32([0]), 16, 2)
+    assert got[2].tolist() == [-1, -1] and ops.device_error() == 2
+    got = ops.paged_update(_i32([0]), _i32([2]), _i32([[-1, -1]]), _i32([0]), _i32([3, 1]), _i32([50]), 16, 2)
+    assert got[2].tolist() == [16, 17] and ops.device_error() == 2  # the list cut to its two entries
+    _no_device_error(ops)
+
+
+# ------------------------------------------------------------------ append
+def _rope_tables(n, D, dtype):
+    inv = 1e6 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)
+    a = torch.arange(n, dtype=torch.float64)[:, None] * inv[None]
+    return a.cos().to(dtype).cuda(), a.sin().to(dtype).cuda()
+
+
+@pytest.mark.parametrize("T,Hq,Hkv,D,page,dtype", [(1, 28, 4, 128, 16, BF), (80, 28, 4, 128, 64, BF),
+                                                    (333, 7, 1, 128, 256, FP), (1001, 16, 16, 64, 32, FP),
+                                                    (17, 40, 8, 64, 128, BF), (5, 96, 32, 128, 16, BF)])
+def test_append(ops, T, Hq, Hkv, D, page, dtype):
+    g = torch.Generator().manual_seed(T)
+    num_pages, max_pos = -(-T // page) + 4, 5000
+    cos, sin = _rope_tables(max_pos, D, dtype)
+    qkv = torch.randn(T, (Hq + 2 * Hkv) * D, generator=g).to(dtype).cuda()
+    pos = torch.randint(0, max_pos, (T,), generator=g).int()
+    slots = torch.randperm(num_pages * page, generator=g)[:T].int()
+    if T > 4:
+        pos[2], slots[2] = -1, -1      # no token here
+        slots[4] = -1                  # rotated, not stored
+    k = torch.full((num_pages, Hkv, page, D), 5.0, dtype=dtype, device="cuda")
+    v, q = torch.full_like(k, 6.0), torch.full((T, Hq, D), 4.0, dtype=dtype, device="cuda")
+    assert ops.paged_rope_append(qkv, pos.cuda(), slots.cuda(), cos, sin, q, k, v) is q
+    x = qkv.double().view(T, -1, D)
+    c, s = cos.double()[pos.clamp(min=0).cuda().long()][:, None], sin.double()[pos.clamp(min=0).cuda().long()][:, None]
+    lo, hi = x[..., :D // 2], x[..., D // 2:]
+    y = torch.cat([lo * c - hi * s, hi * c + lo * s], -1)
+    # one rounding to dtype after two products and a sum in 32 bits
+    size = torch.cat([(lo * c).abs() + (hi * s).abs(), (hi * c).abs() + (lo * s).abs()], -1)
+    tol = torch.finfo(dtype).eps / 2 * y.abs() * 1.001 + 3 * 2.0 ** -24 * size + (2.0 ** -25 if dtype == FP else 0)
+    have = (pos >= 0).cuda()
+    assert ((q.double() - y[:, :Hq]).abs() <= tol[:, :Hq])[have].all()
+    assert (q[~have] == 4).all()
+    rows = k.permute(0, 2, 1, 3).reshape(-1, Hkv, D), v.permute(0, 2, 1, 3).reshape(-1, Hkv, D)
+    kept = (slots >= 0).cuda()
+    at = slots.cuda().long()[kept]
+    assert ((rows[0][at].double() - y[kept][:, Hq:Hq + Hkv]).abs() <= tol[kept][:, Hq:Hq + Hkv]).all()
+    assert torch.equal(rows[1][at], qkv.view(T, -1, D)[kept][:, Hq + Hkv:])
+    other = torch.ones(num_pages * page, dtype=torch.bool, device="cuda")
+    other[at] = False
+    assert (rows[0][other] == 5).all() and (rows[1][other] == 6).all()
+    _no_device_error(ops)
+
+
+def test_append_reports_out_of_range(ops):
+    cos, sin = _rope_tables(10, 64, BF)
+    qkv = torch.randn(3, 3 * 64, device="cuda").to(BF)
+    k = torch.zeros(2, 1, 16, 64, dtype=BF, device="cuda")
+    v, q = torch.zeros_like(k), torch.zeros(3, 1, 64, dtype=BF, device="cuda")
+    ops.paged_rope_append(qkv, _i32([0, 10, 2]), _i32([0, 1, 32]), cos, sin, q, k, v)
+    assert ops.device_error() == 2
+    assert torch.equal(v[0, 0, :2], qkv[:2, 128:]) and (v.view(-1, 64)[2:] == 0).all()
+    last = torch.zeros_like(q)
+    ops.paged_rope_append(qkv, _i32([0, 9, 2]), _i32([-1, -1, -1]), cos, sin, last, k, v)
+    assert torch.equal(last[1], q[1])  # read as the last position
+    _no_device_error(ops)
