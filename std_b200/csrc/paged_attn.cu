@@ -6,10 +6,9 @@
 //
 // Tiles.  The G = Hq / Hkv query heads of a KV head share its keys, so rows
 // are (token, head of the group) pairs: row = t * G + g, TQ = floor(128 / G)
-// whole tokens per 128-row MMA tile.  An item is one KV head's span of up to
-// 2 TQ tokens of one request ("pair": two tiles that share every K/V block) or,
-// when at most TQ tokens are left, one tile ("single").  Keys come in blocks of
-// 128:
+// whole tokens per 128-row tile.  An item is one KV head's span of up to 2 TQ
+// tokens of one request: a pair of tiles that share every K/V block or, when at
+// most TQ tokens are left, a single one.  Keys come in blocks of 128.
 //   S = Q K^T     tcgen05.mma M=128 N=128, Q and K from shared memory
 //   P = exp2(S * scale * log2e - m), 16 bits, written over S in TMEM
 //   O += P V      tcgen05.mma with P as the A operand in TMEM, V MN-major
@@ -19,6 +18,14 @@
 // one stream's MMAs run while the other's softmax does.  The running maximum
 // is raised lazily, when a block passes it by more than 2^8, so O is normally
 // not touched between blocks.
+//
+// Few rows.  A single item of at most 64 rows (decoding: G rows) is computed
+// transposed, keys on the 128 MMA rows and the query rows on N:
+//   S^T = K Q^T    M=128 (keys) N=16, 32 or 64, both operands in shared memory
+//   O^T += V^T P^T M=128 (head dims), A = V MN-major, B = P^T in shared memory
+// A softmax thread then owns one key and N rows, so a block costs N exponentials
+// a thread on all 128 threads instead of 128 on the few threads that have a row,
+// and the MMAs are N wide instead of 128.
 //
 // Split.  One CTA per SM.  The items' costs (blocks, weighted) are laid end to
 // end and cut into equal shares, one per CTA, at block boundaries; a CTA reads
@@ -37,23 +44,32 @@
 // not added to, and their V rows are cleared before the product.
 #include "common.cuh"
 
+#include <type_traits>
+
 namespace stdb {
 
 constexpr int PA_CTAS = 148;     // one CTA per SM
-constexpr int PA_THREADS = 384;  // 2 softmax warpgroups; TMA, MMA and scheduler warp, one idle
+constexpr int PA_THREADS = 384;  // 2 softmax warpgroups; TMA, MMA, scheduler and clearing warp
 // Registers after the split: 2 * 128 * 208 + 128 * 88 = 384 * 168, the launch's total.
 constexpr int PA_REGS_SOFTMAX = 208, PA_REGS_OTHER = 88;
 constexpr int PA_BN = 128;       // keys per block
 constexpr float PA_RESCALE = 8.0f;  // log2 units
 constexpr int PA_W1 = 2, PA_W2 = 3;  // cost of a block in a single and in a pair
 
+// Shared memory: two query slots and a ring of K/V blocks.  A slot holds a
+// 128-row Q tile (halves of 64 columns, 16 KB apart), or, for few rows, a 64-row
+// one (halves 8 KB apart) in its first 16 KB and P^T of stream = slot (a 128-byte
+// row per key) in its last 16 KB.
+constexpr uint32_t PA_SLOT = 32768, PA_PT = 16384;
 template <int D>
 struct PagedTile {
   static constexpr uint32_t kv_bytes = PA_BN * D * 2;
-  static constexpr uint32_t q_bytes = 128 * D * 2;
   static constexpr int stages = D == 128 ? 5 : 8;
-  static constexpr uint32_t smem = 2 * q_bytes + stages * kv_bytes + 1024;
+  static constexpr uint32_t smem = 2 * PA_SLOT + stages * kv_bytes + 1024;
 };
+constexpr int PA_FEW = 64;  // most rows of an item that is computed transposed
+constexpr float PA_LOW = -1e30f;  // few rows: m before the first key
+constexpr int PA_POLY = 4;  // every 4th pair of exponentials on the FMA pipe
 
 // What a CTA leaves for the merge about the item that its share ends inside.
 struct PagedSplit {
@@ -67,7 +83,7 @@ struct PagedAttnParams {
   const int32_t* table;  // [B, width]
   const int32_t* cu_q;   // [B + 1]
   const int32_t* kv_lens;
-  int T, B, width, page, num_pages, Hq, Hkv, G, TQ, causal;
+  int T, B, width, page_log2, num_pages, Hq, Hkv, G, TQ, TQ_few, causal;  // TQ_few = floor(64 / G)
   float scale_log2;
   void* out;   // [T, Hq, D]
   float* lse;  // [T, Hq], may be null
@@ -76,20 +92,14 @@ struct PagedAttnParams {
   PagedSplit* splits;  // [PA_CTAS]
 };
 
-// One request's place: token rows [q0, q0 + n) and kv keys.  Lengths that do
-// not fit the tensors are cut (and reported once, by CTA 0).
-STD_DEV void paged_request(const PagedAttnParams& p, int b, int& q0, int& n, int& kv) {
-  q0 = __ldg(p.cu_q + b);
-  const int q1 = __ldg(p.cu_q + b + 1);
-  kv = __ldg(p.kv_lens + b);
-  n = q1 - q0;
-  if (q0 < 0 || q1 > p.T || n < 0) n = 0;
-  const int room = p.width * p.page;
+// One request's place from its raw entries: token rows [q0, q0 + n), kv keys.
+// Lengths that do not fit the tensors are cut; false: they were.
+STD_DEV bool paged_request(const PagedAttnParams& p, int q0, int q1, int& kv, int& n) {
+  const int room = p.width << p.page_log2;
+  const bool fit = q0 >= 0 && q1 <= p.T && q1 >= q0 && kv >= 0 && kv <= room;
+  n = q0 < 0 || q1 > p.T || q1 < q0 ? 0 : q1 - q0;
   kv = kv < 0 ? 0 : (kv > room ? room : kv);
-}
-STD_DEV bool paged_request_bad(const PagedAttnParams& p, int b) {
-  const int q0 = p.cu_q[b], q1 = p.cu_q[b + 1], kv = p.kv_lens[b];
-  return q0 < 0 || q1 > p.T || q1 < q0 || kv < 0 || kv > p.width * p.page;
+  return fit;
 }
 // Item i of a request: its tokens, the last key that any of them sees (+1).
 STD_DEV void paged_item(const PagedAttnParams& p, int n, int kv, int i, int& t0, int& nt, int& limit, int& nb, int& w) {
@@ -98,6 +108,9 @@ STD_DEV void paged_item(const PagedAttnParams& p, int n, int kv, int i, int& t0,
   limit = p.causal ? max(0, kv - n + t0 + nt) : kv;
   nb = max(1, (limit + PA_BN - 1) / PA_BN);
   w = nt > p.TQ ? PA_W2 : PA_W1;
+}
+STD_DEV int paged_ceil_w(long long x, int w) {
+  return static_cast<int>(w == PA_W1 ? (x + PA_W1 - 1) / PA_W1 : (x + PA_W2 - 1) / PA_W2);
 }
 
 // A piece as the other warps see it: nblk blocks from block j0 of one item.
@@ -123,7 +136,9 @@ struct PagedWalk {
   long long cut;       // cost of the item up to the end of this piece
 
   STD_DEV void request(const PagedAttnParams& p) {
-    paged_request(p, b, q0, n, kv);
+    q0 = __ldg(p.cu_q + b);
+    kv = __ldg(p.kv_lens + b);
+    paged_request(p, q0, __ldg(p.cu_q + b + 1), kv, n);
     items = (n + 2 * p.TQ - 1) / (2 * p.TQ);
   }
   // Advance to the next non-empty piece; false at the end of the share.
@@ -140,8 +155,8 @@ struct PagedWalk {
       paged_item(p, n, kv, i, t0, nt, limit, nb, w);
       const long long cost = static_cast<long long>(nb) * w;
       const long long end = min(cost, skip + rem);
-      j0 = static_cast<int>((skip + w - 1) / w);
-      j1 = static_cast<int>((end + w - 1) / w);
+      j0 = paged_ceil_w(skip, w);
+      j1 = paged_ceil_w(end, w);
       rem -= end - skip;
       skip = 0;
       cut = end;
@@ -152,17 +167,14 @@ struct PagedWalk {
   }
 };
 
+// Instruction descriptor for operands of type T (format 1 = bf16, 0 = fp16).
 template <typename T>
-__host__ __device__ constexpr uint32_t paged_idesc(int M, int N, int b_mn_major);
-template <>
-__host__ __device__ constexpr uint32_t paged_idesc<__nv_bfloat16>(int M, int N, int b_mn_major) {
-  return idesc_bf16_f32(M, N, 0, b_mn_major);
+__host__ __device__ constexpr uint32_t paged_idesc(int M, int N, int a_mn_major, int b_mn_major) {
+  return idesc_bf16_f32(M, N, a_mn_major, b_mn_major) &
+         (std::is_same<T, __half>::value ? ~((1u << 7) | (1u << 10)) : ~0u);
 }
-template <>
-__host__ __device__ constexpr uint32_t paged_idesc<__half>(int M, int N, int b_mn_major) {
-  // A and B formats 0 = fp16
-  return idesc_bf16_f32(M, N, 0, b_mn_major) & ~((1u << 7) | (1u << 10));
-}
+// MMA columns for `rows` few rows.
+STD_DEV int paged_few_cols(int rows) { return rows <= 16 ? 16 : (rows <= 32 ? 32 : 64); }
 
 STD_DEV void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
   asm volatile(
@@ -172,9 +184,430 @@ STD_DEV void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, 
       : "memory");
 }
 
+// Static shared memory of a CTA with an ST-stage ring.
+template <int ST>
+struct PagedShared {
+  uint64_t bar_q_full[2], bar_q_empty[2];        // query slots
+  uint64_t bar_full[ST], bar_empty[ST];          // K/V ring
+  uint64_t bar_s[2], bar_p[2], bar_p2[2], bar_o[2];  // per stream: S there, P's halves there, O complete
+  uint64_t bar_join, bar_joined;                 // a single's two streams
+  uint64_t bar_group[2];                         // few rows: the four warps of a stream
+  uint64_t bar_piece[PA_PIECES], bar_taken[PA_PIECES];
+  uint64_t bar_tail, bar_fix;                    // a tail's V there, its rows cleared
+  uint64_t bar_end;
+  // A single's statistics, of one use at a time: whole tiles hand them from
+  // stream 1 to stream 0, few rows keep theirs here.  A stream's warps write the
+  // next piece's only after a barrier that all readers of the last have passed.
+  union {
+    struct {
+      float m[128], l[128];
+    };
+    struct {
+      alignas(16) float ref[2][PA_FEW];    // m of each stream and row; the streams' weights at the join
+      alignas(16) float alpha[2][PA_FEW];  // the factor of a rescaled O
+    };
+  };
+  alignas(16) int flag[2][2][4];  // few rows: a vote per warp, by step parity
+  PagedPiece piece[PA_PIECES];
+  uint32_t tmem;
+};
+
+STD_DEV void tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+STD_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+template <int N>
+STD_DEV void tmem_ld_cols(uint32_t taddr, uint32_t* r) {
+  if constexpr (N == 16) {
+    tmem_ld16(taddr, r);
+  } else {
+#pragma unroll
+    for (int c = 0; c < N / 32; ++c) tmem_ld32(taddr + 32 * c, r + 32 * c);
+  }
+}
+template <int N>
+STD_DEV void tmem_st_cols(uint32_t taddr, const uint32_t* r) {
+  if constexpr (N == 16) {
+    tmem_st16(taddr, r);
+  } else {
+#pragma unroll
+    for (int c = 0; c < N / 32; ++c) tmem_st32(taddr + 32 * c, r + 32 * c);
+  }
+}
+// One thread of a converged warp, the same one each time.  Behind this predicate
+// (not behind lane == 0) the compiler knows that a single thread runs and feeds
+// tcgen05.mma its uniform registers directly; otherwise it serialises over
+// possible threads, ~170 cycles an MMA.
+STD_DEV bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+// Largest value of the warp (NaN ignored).
+STD_DEV float warp_max_redux(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+// Two floats in one 64-bit register, for the paired FMA and add.
+STD_DEV uint64_t f2_make(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+STD_DEV float2 f2_split(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+STD_DEV uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+STD_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+STD_DEV float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// 2^y for two y <= 127 on the FMA and integer pipes, to spare the SFU (16
+// results a cycle and SM): y = n + f with n whole and |f| <= 1/2, 2^f = 1 + f q(f)
+// with q the degree-4 polynomial that interpolates (2^f - 1) / f at the Chebyshev
+// nodes of [-1/2, 1/2] (off by at most 2.1e-7, 2.6e-7 as rounded here), n added
+// to the exponent.  At and below -127 (masked: -inf) the sum is exactly 0, since
+// 2^0 is exactly 1 here; between that and -126 a number below 2^-126.
+STD_DEV float2 ex2_fma2(uint64_t y2) {
+  float2 y = f2_split(y2);
+  y.x = fmaxf(y.x, -127.f);
+  y.y = fmaxf(y.y, -127.f);
+  const float MAGIC = 12582912.f;  // 1.5 * 2^23: adding it leaves round(y) in the low bits
+  const uint64_t v = f2_make(y.x, y.y);
+  const uint64_t t = f2_add(v, f2_make(MAGIC, MAGIC));
+  const uint64_t n = f2_add(t, f2_make(-MAGIC, -MAGIC));
+  const uint64_t f = f2_fma(n, f2_make(-1.f, -1.f), v);
+  uint64_t r = f2_make(1.338130254e-03f, 1.338130254e-03f);
+  r = f2_fma(r, f, f2_make(9.666368515e-03f, 9.666368515e-03f));
+  r = f2_fma(r, f, f2_make(5.550381014e-02f, 5.550381014e-02f));
+  r = f2_fma(r, f, f2_make(2.402234904e-01f, 2.402234904e-01f));
+  r = f2_fma(r, f, f2_make(6.931471806e-01f, 6.931471806e-01f));
+  r = f2_fma(r, f, f2_make(1.f, 1.f));
+  const float2 e = f2_split(r), k = f2_split(t);
+  float2 out;
+  out.x = __uint_as_float(__float_as_uint(e.x) + (__float_as_uint(k.x) << 23));
+  out.y = __uint_as_float(__float_as_uint(e.y) + (__float_as_uint(k.y) << 23));
+  return out;
+}
+
+// One step of a whole tile's softmax: S (128 columns of this thread's row) to
+// P, with the row's running m and l.  Raises sh's barriers for P's halves.
+template <typename T, int D>
+STD_DEV void paged_softmax_step(uint32_t tS, uint32_t tO, float sc, int nvis, float& m_run, float& l_run,
+                                uint64_t* bar_p, uint64_t* bar_p2, int lane) {
+  uint32_t x[PA_BN];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, x + c * 32);
+  tmem_wait_ld();
+  if (__any_sync(0xffffffffu, nvis < PA_BN)) {
+#pragma unroll
+    for (int j = 0; j < PA_BN; ++j)
+      if (j >= nvis) x[j] = 0xff800000u;  // -inf
+  }
+  float m4[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) m4[c] = fmaxf(__uint_as_float(x[c]), __uint_as_float(x[4 + c]));
+#pragma unroll
+  for (int j = 8; j < PA_BN; j += 8)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) m4[c] = max3(m4[c], __uint_as_float(x[j + c]), __uint_as_float(x[j + 4 + c]));
+  const float m_c = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;  // scale > 0
+  // This block's S is issued after the stream's previous P V, and its barrier
+  // covers all MMAs before it: O is at rest here.
+  const bool need = m_run != -INFINITY && m_c > m_run + PA_RESCALE;
+  if (__any_sync(0xffffffffu, need)) {
+    const float alpha = need ? exp2f(m_run - m_c) : 1.0f;
+    uint32_t o[32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      tmem_ld32(tO + c * 32, o);
+      tmem_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+      tmem_st32(tO + c * 32, o);
+    }
+    if (need) {
+      l_run *= alpha;
+      m_run = m_c;
+    }
+  }
+  if (m_run == -INFINITY) m_run = m_c;
+  // a row that has seen no key yet keeps P = 2^-inf = 0
+  const float nm = m_run == -INFINITY ? 0.f : -m_run;
+  const uint64_t sc2 = f2_make(sc, sc), nm2 = f2_make(nm, nm);
+  uint64_t l2[2] = {f2_make(l_run, 0.f), f2_make(0.f, 0.f)};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const uint64_t y = f2_fma(f2_make(__uint_as_float(x[c * 32 + 2 * j]), __uint_as_float(x[c * 32 + 2 * j + 1])), sc2, nm2);
+      float2 e;
+      if (PA_POLY > 0 && j % PA_POLY == PA_POLY - 1) {
+        e = ex2_fma2(y);
+      } else {
+        e = f2_split(y);
+        e.x = ex2_approx(e.x);
+        e.y = ex2_approx(e.y);
+      }
+      l2[j & 1] = f2_add(l2[j & 1], f2_make(e.x, e.y));
+      pk[j] = pack_pair<T>(e.x, e.y);
+    }
+    tmem_st16(tS + c * 16, pk);
+    if (c & 1) {
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(c == 1 ? bar_p : bar_p2);
+    }
+  }
+  const float2 l = f2_split(f2_add(l2[0], l2[1]));
+  l_run = l.x + l.y;
+}
+
+// A piece with few rows, for one warp of stream s (thread = key of the block,
+// N >= the piece's rows columns).  ns, no, nj, ng: phases used so far of the
+// stream's S, O, join and group barriers; bar_q_empty: its query slot's.  False when a wait ran out.
+template <typename T, int D, int N, int ST>
+STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, PagedShared<ST>& sh, uint8_t* sQ,
+                             uint32_t tS, uint32_t tO, int s, uint64_t* bar_q_empty, uint32_t& ns, uint32_t& no, uint32_t& nj,
+                             uint32_t& ng) {
+  const int tid = threadIdx.x, lane = tid & 31, w = (tid >> 5) & 3, key = tid & 127;
+  const int rows = piece.tokens * p.G, steps = (piece.nblk - s + 1) >> 1;
+  const float sc = p.scale_log2;
+  uint8_t* row_p = sQ + s * PA_SLOT + PA_PT + key * 128;
+  // [warp][row] values of a stream's warps, where P is not needed (P V done)
+  auto red = [&](int stream, int warp, int n) -> float& {
+    return reinterpret_cast<float*>(sQ + stream * PA_SLOT + PA_PT)[warp * PA_FEW + n];
+  };
+  auto group_sync = [&]() -> bool {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.bar_group[s]);
+    return __all_sync(0xffffffffu, mbar_wait(&sh.bar_group[s], ng++ & 1));
+  };
+  float l[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) l[n] = 0.f;
+  const int all_see = p.causal ? min(piece.limit, piece.first) : piece.limit;  // keys that every row sees
+  for (int k = 0; k < steps; ++k, ++ns) {
+    if (!__all_sync(0xffffffffu, mbar_wait(&sh.bar_s[s], ns & 1))) return false;
+    tc_fence_after();
+    const int pos = (piece.j0 + 2 * k + s) * PA_BN + key;
+    float x[N];
+    // scores, -inf where hidden and in the columns past the last row
+    auto load = [&]() {
+      tmem_ld_cols<N>(tS, reinterpret_cast<uint32_t*>(x));
+      tmem_wait_ld();
+      if (__any_sync(0xffffffffu, pos >= all_see)) {
+        int see = p.causal ? min(piece.limit, piece.first) : piece.limit, g = 0;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          if (pos >= see || n >= rows) x[n] = -INFINITY;
+          if (++g == p.G) {
+            g = 0;
+            if (p.causal) see = min(piece.limit, see + 1);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+          if (n >= rows) x[n] = -INFINITY;
+      }
+    };
+    load();
+    bool fresh = k == 0;  // m has to be found (first block) or raised
+    if (k > 0) {
+      float over = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < N; n += 4) {
+        const float4 m = *reinterpret_cast<const float4*>(&sh.ref[s][n]);
+        x[n] = fmaf(x[n], sc, -m.x);
+        x[n + 1] = fmaf(x[n + 1], sc, -m.y);
+        x[n + 2] = fmaf(x[n + 2], sc, -m.z);
+        x[n + 3] = fmaf(x[n + 3], sc, -m.w);
+        over = fmaxf(max3(over, x[n], x[n + 1]), fmaxf(x[n + 2], x[n + 3]));
+      }
+      const bool vote = __any_sync(0xffffffffu, over > PA_RESCALE);
+      if (lane == 0) sh.flag[s][k & 1][w] = vote ? 1 : 0;
+      if (!group_sync()) return false;
+      const int4 f = *reinterpret_cast<const int4*>(sh.flag[s][k & 1]);
+      fresh = (f.x | f.y | f.z | f.w) != 0;
+      if (fresh) load();
+    }
+    if (fresh) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        const float v = warp_max_redux(x[n]);
+        if (lane == (n & 31)) red(s, w, n) = v;
+      }
+      if (!group_sync()) return false;
+      if (key < N) {
+        const float mx =
+            fmaxf(fmaxf(red(s, 0, key), red(s, 1, key)), fmaxf(red(s, 2, key), red(s, 3, key))) * sc;
+        const float old = k == 0 ? PA_LOW : sh.ref[s][key];
+        const float m = mx > old + PA_RESCALE ? mx : old;
+        sh.alpha[s][key] = exp2f(old - m);
+        sh.ref[s][key] = m;
+      }
+      if (!group_sync()) return false;
+      if (k > 0) {
+        uint32_t o[16];
+#pragma unroll
+        for (int c = 0; c < N; c += 16) {
+          tmem_ld16(tO + c, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float a = sh.alpha[s][c + j];
+            l[c + j] *= a;
+            o[j] = __float_as_uint(__uint_as_float(o[j]) * a);
+          }
+          tmem_st16(tO + c, o);
+        }
+        tmem_wait_st();
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n) x[n] = fmaf(x[n], sc, -sh.ref[s][n]);
+    }
+#pragma unroll
+    for (int n = 0; n < N; n += 8) {
+      float e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        e[j] = ex2_approx(x[n + j]);
+        l[n + j] += e[j];
+      }
+      *reinterpret_cast<uint4*>(row_p + (((n >> 3) ^ (key & 7)) << 4)) =
+          make_uint4(pack_pair<T>(e[0], e[1]), pack_pair<T>(e[2], e[3]), pack_pair<T>(e[4], e[5]),
+                     pack_pair<T>(e[6], e[7]));
+    }
+    fence_async_smem();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.bar_p[s]);
+  }
+  if (steps > 0) {
+    if (!__all_sync(0xffffffffu, mbar_wait(&sh.bar_o[s], no++ & 1))) return false;
+    // sum of l over the warp's keys, halving the rows a lane keeps at each step
+    int base = 0;
+#pragma unroll
+    for (int o = 16, half = N / 2; o > 0; o >>= 1, half >>= 1) {
+      if (half > 0) {
+        const bool up = (lane & o) != 0;
+        base += up ? half : 0;
+#pragma unroll
+        for (int i = 0; i < (half > 0 ? half : 1); ++i) {
+          const float give = up ? l[i] : l[i + half], keep = up ? l[i + half] : l[i];
+          l[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+      } else {
+        l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+      }
+    }
+    red(s, w, base) = l[0];
+    if (N == 64) red(s, w, base + 1) = l[1];
+    fence_async_smem();  // (a TMA load may write here next)
+  }
+  if (s == 1) {
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.bar_join);
+    if (!__all_sync(0xffffffffu, mbar_wait(&sh.bar_joined, nj++ & 1))) return false;
+    // stream 0 is done too, and with it the query slot, P in it included
+    if (tid == 128) mbar_arrive(bar_q_empty);
+    return true;
+  }
+  if (!group_sync() || !__all_sync(0xffffffffu, mbar_wait(&sh.bar_join, nj++ & 1))) return false;
+  const bool whole = piece.slot < 0, two = piece.nblk > 1;
+  const size_t orow0 = static_cast<size_t>(piece.token0) * p.Hq + piece.h * p.G;
+  if (key < N) {
+    const float la = red(0, 0, key) + red(0, 1, key) + red(0, 2, key) + red(0, 3, key);
+    const float lb = two ? red(1, 0, key) + red(1, 1, key) + red(1, 2, key) + red(1, 3, key) : 0.f;
+    const float ma = sh.ref[0][key], mb = two ? sh.ref[1][key] : PA_LOW, m = fmaxf(ma, mb);
+    const float wa = la != 0.f ? exp2f(ma - m) : 0.f, wb = lb != 0.f ? exp2f(mb - m) : 0.f;
+    const float lt = (la != 0.f ? la * wa : 0.f) + (lb != 0.f ? lb * wb : 0.f);
+    const float inv = whole && lt != 0.f ? 1.f / lt : 1.f;
+    sh.ref[0][key] = wa * inv;
+    sh.ref[1][key] = wb * inv;
+    if (key < rows) {
+      if (!whole)
+        p.ws_ml[static_cast<size_t>(piece.slot) * 256 + key] = make_float2(lt != 0.f ? m : -INFINITY, lt);
+      else if (p.lse != nullptr)
+        p.lse[orow0 + static_cast<size_t>(key / p.G) * p.Hq + key % p.G] =
+            lt != 0.f ? (m + log2f(lt)) * 0.69314718055994530942f : -INFINITY;
+    }
+  }
+  if (!group_sync()) return false;
+  tc_fence_after();
+  // thread = head dim: O^T's columns are rows
+  size_t orow = orow0;
+  int g = 0;
+#pragma unroll
+  for (int c = 0; c < N; c += 16) {
+    if (c < rows) {
+      uint32_t oa[16], ob[16];
+      tmem_ld16(tO + c, oa);
+      if (two) tmem_ld16(tO + 128 + c, ob);
+      tmem_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float wa = sh.ref[0][c + j], wb = sh.ref[1][c + j];
+        float v = wa != 0.f ? __uint_as_float(oa[j]) * wa : 0.f;
+        if (two) v += wb != 0.f ? __uint_as_float(ob[j]) * wb : 0.f;
+        if (c + j < rows && key < D) {
+          if (whole)
+            static_cast<T*>(p.out)[orow * D + key] = to_type<T>(v);
+          else
+            p.ws_o[(static_cast<size_t>(piece.slot) * 256 + c + j) * D + key] = v;
+        }
+        ++orow;
+        if (++g == p.G) {
+          g = 0;
+          orow += p.Hq - p.G;
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(&sh.bar_joined);
+  return true;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(PA_THREADS, 1)
-    paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+    paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ,
+                      const __grid_constant__ CUtensorMap tmQfew, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const PagedAttnParams p) {
   typedef PagedTile<D> Tile;
   constexpr int ST = Tile::stages;
@@ -184,144 +617,58 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sQ = smem;                     // [2][q_bytes]
-  uint8_t* sKV = smem + 2 * Tile::q_bytes;  // [ST][kv_bytes]
-  __shared__ __align__(8) uint64_t bar_q_full[2], bar_q_empty[2], bar_full[ST], bar_empty[ST], bar_s[2], bar_p[2],
-      bar_o[2], bar_join, bar_joined, bar_piece[PA_PIECES], bar_taken[PA_PIECES], bar_end;
-  __shared__ PagedPiece s_piece[PA_PIECES];
-  __shared__ uint32_t s_tmem;
-  __shared__ float s_m[128], s_l[128];
-  __shared__ long long s_warp[PA_THREADS / 32], s_off;
-  __shared__ int s_b;
+  uint8_t* sQ = smem;                 // [2][PA_SLOT]
+  uint8_t* sKV = smem + 2 * PA_SLOT;  // [ST][kv_bytes]
+  __shared__ PagedShared<ST> sh;
 
   if (tid == 256) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar_q_full[i], 1);
-      mbar_init(&bar_q_empty[i], 1);
-      mbar_init(&bar_s[i], 1);
-      mbar_init(&bar_p[i], 4);
-      mbar_init(&bar_o[i], 1);
+      mbar_init(&sh.bar_q_full[i], 1);
+      mbar_init(&sh.bar_q_empty[i], 1);
+      mbar_init(&sh.bar_s[i], 1);
+      mbar_init(&sh.bar_p[i], 4);
+      mbar_init(&sh.bar_o[i], 1);
+      mbar_init(&sh.bar_p2[i], 4);
+      mbar_init(&sh.bar_group[i], 4);
     }
     for (int i = 0; i < ST; ++i) {
-      mbar_init(&bar_full[i], 1);
-      mbar_init(&bar_empty[i], 1);
+      mbar_init(&sh.bar_full[i], 1);
+      mbar_init(&sh.bar_empty[i], 1);
     }
     for (int i = 0; i < PA_PIECES; ++i) {
-      mbar_init(&bar_piece[i], 1);
-      mbar_init(&bar_taken[i], 10);  // the warps that read it
+      mbar_init(&sh.bar_piece[i], 1);
+      mbar_init(&sh.bar_taken[i], 11);  // the warps that read it
     }
-    mbar_init(&bar_join, 4);
-    mbar_init(&bar_joined, 4);
-    mbar_init(&bar_end, 1);
+    mbar_init(&sh.bar_join, 4);
+    mbar_init(&sh.bar_joined, 4);
+    mbar_init(&sh.bar_end, 1);
+    mbar_init(&sh.bar_tail, 1);
+    mbar_init(&sh.bar_fix, 1);
     fence_barrier_init();
     prefetch_tensormap(&tmQ);
     prefetch_tensormap(&tmK);
     prefetch_tensormap(&tmV);
-    s_b = -1;
   }
   pdl_wait();
   if (warp == 9) {
-    tmem_alloc(&s_tmem, 512);
+    tmem_alloc(&sh.tmem, 512);
     tmem_relinquish();
   }
 
-  // ---------------- this CTA's share of the blocks ----------------
-  // cost of a request: its items' blocks, for all KV heads.  Requests of
-  // several items are summed by the whole warp.
-  auto request_cost = [&](int b) -> long long {
-    int q0 = 0, n = 0, kv = 0;
-    if (b < p.B) {
-      paged_request(p, b, q0, n, kv);
-      if (cta == 0 && paged_request_bad(p, b)) std_set_error(STD_DEVERR_LENGTH);
-    }
-    const int items = (n + 2 * p.TQ - 1) / (2 * p.TQ);
-    int t0, nt, limit, nb, w;
-    long long cost = 0;
-    if (items == 1) {
-      paged_item(p, n, kv, 0, t0, nt, limit, nb, w);
-      cost = static_cast<long long>(nb) * w;
-    }
-    for (uint32_t many = __ballot_sync(0xffffffffu, items > 1); many != 0; many &= many - 1) {
-      const int src = __ffs(many) - 1;
-      const int n_ = __shfl_sync(0xffffffffu, n, src), kv_ = __shfl_sync(0xffffffffu, kv, src);
-      const int items_ = __shfl_sync(0xffffffffu, items, src);
-      long long sum = 0;
-      for (int i = lane; i < items_; i += 32) {
-        paged_item(p, n_, kv_, i, t0, nt, limit, nb, w);
-        sum += static_cast<long long>(nb) * w;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == src) cost = sum;
-    }
-    return cost * p.Hkv;
-  };
-  long long total = 0, mine = 0, before = 0;  // before: cost of the requests ahead of this thread's
-  for (int b0 = 0; b0 < p.B; b0 += PA_THREADS) {
-    mine = request_cost(b0 + tid);
-    long long inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += u;
-    }
-    if (lane == 31) s_warp[warp] = inc;
-    __syncthreads();
-    before = total + inc - mine;
-    for (int w = 0; w < PA_THREADS / 32; ++w) {
-      if (w < warp) before += s_warp[w];
-      total += s_warp[w];
-    }
-    __syncthreads();
-  }
-  long long share = (total + PA_CTAS - 1) / PA_CTAS;
-  share = max(share, static_cast<long long>(2 * PA_W2));
-  const long long x0 = share * cta;
-  if (x0 < total) {
-    if (p.B <= PA_THREADS) {
-      if (x0 >= before && x0 < before + mine) {
-        s_b = tid;
-        s_off = x0 - before;
-      }
-    } else {  // a second pass over the requests, in chunks
-      long long run = 0;
-      for (int b0 = 0; b0 < p.B; b0 += PA_THREADS) {
-        const long long c = request_cost(b0 + tid);
-        long long inc = c;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const long long u = __shfl_up_sync(0xffffffffu, inc, o);
-          if (lane >= o) inc += u;
-        }
-        if (lane == 31) s_warp[warp] = inc;
-        __syncthreads();
-        long long at = run + inc - c;
-        for (int w = 0; w < PA_THREADS / 32; ++w) {
-          if (w < warp) at += s_warp[w];
-          run += s_warp[w];
-        }
-        if (x0 >= at && x0 < at + c) {
-          s_b = b0 + tid;
-          s_off = x0 - at;
-        }
-        __syncthreads();
-      }
-    }
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = sh.tmem;
   // Dependents may launch only once this CTA holds its TMEM (verify_attn.cu).
   pdl_launch_dependents();
 
   // The next piece; false when there is none (or its wait ran out).
   auto next_piece = [&](uint32_t& n, PagedPiece& piece) -> bool {
     const int i = n % PA_PIECES;
-    if (!__all_sync(0xffffffffu, mbar_wait(&bar_piece[i], (n / PA_PIECES) & 1))) return false;
-    piece = s_piece[i];
+    if (!__all_sync(0xffffffffu, mbar_wait(&sh.bar_piece[i], (n / PA_PIECES) & 1))) return false;
+    piece = sh.piece[i];
     __syncwarp();
-    if (lane == 0) mbar_arrive(&bar_taken[i]);
+    if (lane == 0) mbar_arrive(&sh.bar_taken[i]);
     ++n;
     return piece.nblk > 0;
   };
@@ -334,12 +681,23 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const uint32_t tS = trow + s * 128, tO = trow + T_O + s * 128;
     const int rt = r / p.G, rg = r % p.G;  // token and head of this row in its tile
     const float sc = p.scale_log2;
-    uint32_t npiece = 0, ns = 0, no = 0, nj = 0;  // pieces, steps, results and joins so far
+    uint32_t npiece = 0, ns = 0, no = 0, nj = 0, ng = 0, nq = 0;  // pieces, steps, results, joins, group syncs, query tiles so far
     bool ok = true;
     PagedPiece piece;
     while (ok && next_piece(npiece, piece)) {
       const int nblk = piece.nblk;
       const bool pair = piece.tokens > p.TQ;
+      if (piece.tokens <= p.TQ_few) {
+        const int rows = piece.tokens * p.G;
+        if (rows <= 16)
+          ok = paged_few_piece<T, D, 16>(p, piece, sh, sQ, tS, tO, s, &sh.bar_q_empty[nq++ & 1], ns, no, nj, ng);
+        else if (rows <= 32)
+          ok = paged_few_piece<T, D, 32>(p, piece, sh, sQ, tS, tO, s, &sh.bar_q_empty[nq++ & 1], ns, no, nj, ng);
+        else
+          ok = paged_few_piece<T, D, 64>(p, piece, sh, sQ, tS, tO, s, &sh.bar_q_empty[nq++ & 1], ns, no, nj, ng);
+        continue;
+      }
+      nq += pair ? 2 : 1;
       const int tile = pair ? s : 0;
       const int t = tile * p.TQ + rt;  // token of the item
       const bool valid_row = rt < p.TQ && t < piece.tokens;
@@ -349,76 +707,19 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       const int steps = pair ? nblk : (nblk - s + 1) >> 1;
       float m_run = -INFINITY, l_run = 0.f;
       for (int k = 0; k < steps; ++k, ++ns) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&bar_s[s], ns & 1));
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_s[s], ns & 1));
         if (!ok) break;
         if (live) {
           tc_fence_after();
-          uint32_t x[PA_BN];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, x + c * 32);
-          tmem_wait_ld();
           const int nvis = limit - (piece.j0 + (pair ? k : 2 * k + s)) * PA_BN;  // visible keys of this block
-          float mx = -INFINITY;
-          if (__any_sync(0xffffffffu, nvis < PA_BN)) {
-#pragma unroll
-            for (int j = 0; j < PA_BN; ++j) {
-              if (j >= nvis) x[j] = 0xff800000u;  // -inf
-              mx = fmaxf(mx, __uint_as_float(x[j]));
-            }
-          } else {
-            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int j = 0; j < PA_BN; j += 4)
-#pragma unroll
-              for (int c = 0; c < 4; ++c) m4[c] = fmaxf(m4[c], __uint_as_float(x[j + c]));
-            mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-          }
-          const float m_c = mx * sc;  // scale > 0
-          // This block's S is issued after the stream's previous P V, and its
-          // barrier covers all MMAs before it: O is at rest here.
-          const bool need = m_run != -INFINITY && m_c > m_run + PA_RESCALE;
-          if (__any_sync(0xffffffffu, need)) {
-            const float alpha = need ? exp2f(m_run - m_c) : 1.0f;
-            uint32_t o[32];
-#pragma unroll
-            for (int piece = 0; piece < D / 32; ++piece) {
-              tmem_ld32(tO + piece * 32, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-              tmem_st32(tO + piece * 32, o);
-            }
-            if (need) {
-              l_run *= alpha;
-              m_run = m_c;
-            }
-          }
-          if (m_run == -INFINITY) m_run = m_c;
-          // a row that has seen no key yet: exp2(-inf + 0) = 0 everywhere
-          const float nm = m_run == -INFINITY ? 0.f : -m_run;
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t pk[32];
-            float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float e0 = ex2_approx(fmaf(__uint_as_float(x[c * 64 + 2 * j]), sc, nm));
-              const float e1 = ex2_approx(fmaf(__uint_as_float(x[c * 64 + 2 * j + 1]), sc, nm));
-              l0 += e0;
-              l1 += e1;
-              pk[j] = pack_pair<T>(e0, e1);
-            }
-            l_run += l0 + l1;
-            tmem_st32(tS + c * 32, pk);
-          }
-          tmem_wait_st();
-          tc_fence_before();
+          paged_softmax_step<T, D>(tS, tO, sc, nvis, m_run, l_run, &sh.bar_p[s], &sh.bar_p2[s], lane);
+        } else if (lane == 0) {
+          mbar_arrive(&sh.bar_p[s]);
+          mbar_arrive(&sh.bar_p2[s]);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar_p[s]);
       }
       // ---- the item's result ----
-      if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bar_o[s], no++ & 1));
+      if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_o[s], no++ & 1));
       if (!ok) break;
       float wa = 1.f, wb = 0.f, m = m_run, l = l_run;
       bool join = false;
@@ -426,15 +727,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         // stream 1, its last product done, hands (m, l) to stream 0, which
         // reads both accumulators
         if (s == 1) {
-          s_m[r] = m_run;
-          s_l[r] = l_run;
+          sh.m[r] = m_run;
+          sh.l[r] = l_run;
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bar_join);
+          if (lane == 0) mbar_arrive(&sh.bar_join);
         } else {
-          ok = __all_sync(0xffffffffu, mbar_wait(&bar_join, nj & 1));
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_join, nj & 1));
           if (!ok) break;
-          const float mB = s_m[r], lB = s_l[r];
+          const float mB = sh.m[r], lB = sh.l[r];
           join = __any_sync(0xffffffffu, lB != 0.f);
           m = fmaxf(m_run, mB);
           wa = l_run != 0.f ? exp2f(m_run - m) : 0.f;
@@ -445,7 +746,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       const bool whole = piece.slot < 0;
       if (live && (pair || s == 0)) {
         tc_fence_after();
-        const bool seen = l != 0.f, seen_a = l_run != 0.f, seen_b = join && s_l[r] != 0.f;
+        const bool seen = l != 0.f, seen_a = l_run != 0.f, seen_b = join && sh.l[r] != 0.f;
         const float inv = whole && seen ? 1.f / l : 1.f;
         const int token = piece.token0 + t;
         const int head = piece.h * p.G + rg;
@@ -494,9 +795,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       if (!pair) {
         if (s == 0) {
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bar_joined);
+          if (lane == 0) mbar_arrive(&sh.bar_joined);
         } else {
-          ok = __all_sync(0xffffffffu, mbar_wait(&bar_joined, nj & 1));
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_joined, nj & 1));
         }
         ++nj;
       }
@@ -505,34 +806,37 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_OTHER));
     if (warp == 8) {
       // ---------------- TMA producer: the whole warp, a page per lane ----------------
-      const int box = min(p.page, PA_BN);          // rows per copy
-      const int per_block = PA_BN / box;           // copies per block
+      const int box_log2 = min(p.page_log2, 7), box = 1 << box_log2;  // rows per copy
+      const int per_block = PA_BN >> box_log2;           // copies per block
       const uint32_t copy_bytes = box * D * 2;
-      const int groups = p.page / 8;               // 8-row groups per page and head
+      const int groups = 1 << (p.page_log2 - 3);   // 8-row groups per page and head
       uint32_t nld = 0, nq = 0;                    // loads and Q tiles issued
       uint32_t np = 0;
-      bool ok = true;
+      bool ok = true, was_few = false;
       PagedPiece piece;
       while (ok && next_piece(np, piece)) {
         const int32_t* row = p.table + static_cast<size_t>(piece.b) * p.width;
         const int nblk = piece.nblk, limit = piece.limit;
-        const bool pair = piece.tokens > p.TQ;
-        // queries
+        const bool pair = piece.tokens > p.TQ, few = piece.tokens <= p.TQ_few;
+        // queries; a whole tile may take its slot's last half only when the few-row
+        // piece before it is done there
+        if (was_few && !few) ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_q_empty[(nq - 1) & 1], ((nq - 1) >> 1) & 1));
+        was_few = few;
         for (int s = 0; ok && s < (pair ? 2 : 1); ++s, ++nq) {
           const int st = nq & 1;
-          if (nq >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&bar_q_empty[st], ((nq >> 1) - 1) & 1));
+          if (nq >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_q_empty[st], ((nq >> 1) - 1) & 1));
           if (ok && lane == 0) {
-            mbar_arrive_expect_tx(&bar_q_full[st], p.TQ * p.G * D * 2);
+            mbar_arrive_expect_tx(&sh.bar_q_full[st], (few ? p.TQ_few : p.TQ) * p.G * D * 2);
             for (int hf = 0; hf < HALVES; ++hf)
-              tma_load_4d(sQ + st * Tile::q_bytes + hf * 16384, &tmQ, &bar_q_full[st], hf * 64, 0, piece.h,
-                          piece.token0 + s * p.TQ);
+              tma_load_4d(sQ + st * PA_SLOT + hf * (few ? 8192 : 16384), few ? &tmQfew : &tmQ, &sh.bar_q_full[st], hf * 64,
+                          0, piece.h, piece.token0 + s * p.TQ);
           }
         }
         // the page of copy `lane` of block j (the copies of one page share it)
         auto page_of = [&](int j) -> int {
           const int key = j * PA_BN + lane * box;
           if (lane >= per_block || j >= piece.j0 + nblk || key >= limit) return 0;
-          const int id = __ldg(row + key / p.page);
+          const int id = __ldg(row + (key >> p.page_log2));
           if (id < 0 || id >= p.num_pages) {
             std_set_error(STD_DEVERR_BOUNDS);
             return p.num_pages;  // past the pool: TMA fills zeros
@@ -541,16 +845,16 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         };
         auto load = [&](const CUtensorMap* map, int j, int id) {
           const int st = nld % ST;
-          if (nld >= ST) ok = ok && __all_sync(0xffffffffu, mbar_wait(&bar_empty[st], ((nld / ST) - 1) & 1));
+          if (nld >= ST) ok = ok && __all_sync(0xffffffffu, mbar_wait(&sh.bar_empty[st], ((nld / ST) - 1) & 1));
           if (!ok) return;
           const int left = limit - j * PA_BN;
           const int copies = left <= 0 ? 0 : min(per_block, (left + box - 1) / box);
-          if (lane == 0) mbar_arrive_expect_tx(&bar_full[st], copies * copy_bytes);
+          if (lane == 0) mbar_arrive_expect_tx(&sh.bar_full[st], copies * copy_bytes);
           __syncwarp();
           if (lane < copies) {
             const int key = j * PA_BN + lane * box;
-            const int g = (id * p.Hkv + piece.h) * groups + (key % p.page) / 8;
-            tma_load_4d(sKV + st * Tile::kv_bytes + lane * copy_bytes, map, &bar_full[st], 0, 0, 0,
+            const int g = (id * p.Hkv + piece.h) * groups + ((key & ((1 << p.page_log2) - 1)) >> 3);
+            tma_load_4d(sKV + st * Tile::kv_bytes + lane * copy_bytes, map, &sh.bar_full[st], 0, 0, 0,
                         id >= p.num_pages ? p.num_pages * p.Hkv * groups : g);
           }
           ++nld;
@@ -569,123 +873,273 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
       }
       // never leave a copy in flight
-      for (uint32_t c = nld < ST ? 0 : nld - ST; c < nld; ++c) mbar_wait(&bar_full[c % ST], (c / ST) & 1);
-      for (uint32_t c = nq < 2 ? 0 : nq - 2; c < nq; ++c) mbar_wait(&bar_q_full[c & 1], (c >> 1) & 1);
+      for (uint32_t c = nld < ST ? 0 : nld - ST; c < nld; ++c) mbar_wait(&sh.bar_full[c % ST], (c / ST) & 1);
+      for (uint32_t c = nq < 2 ? 0 : nq - 2; c < nq; ++c) mbar_wait(&sh.bar_q_full[c & 1], (c >> 1) & 1);
     } else if (warp == 9) {
-      // ---------------- MMA issuer (lane 0; the warp clears V rows) ----------------
-      constexpr uint32_t idS = paged_idesc<T>(128, PA_BN, 0);
-      constexpr uint32_t idO = paged_idesc<T>(128, D, 1);
-      uint32_t ld0 = 0, q0 = 0, np[2] = {0, 0};
-      uint32_t npiece = 0;
-      bool ok = true;
-      PagedPiece piece;
-      while (ok && next_piece(npiece, piece)) {
-        const int nblk = piece.nblk;
-        const bool pair = piece.tokens > p.TQ;
-        const int steps = pair ? 2 * nblk : nblk;
-        auto issue_s = [&](int u) {
-          const int s = u & 1;
-          const int k = pair ? u >> 1 : u;
-          const uint32_t c = ld0 + ((pair || k == 0) ? 2 * k : 2 * k - 1), st = c % ST;
-          const uint32_t qi = q0 + (pair ? s : 0), qs = qi & 1;
-          if (ok && (!pair || s == 0)) ok = mbar_wait(&bar_full[st], (c / ST) & 1);
-          if (ok && (u == 0 || (pair && u == 1))) ok = mbar_wait(&bar_q_full[qs], (qi >> 1) & 1);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) return;
-          tc_fence_after();
-          if (lane == 0) {
-            // (a descriptor's low bits are the address / 16, so steps are added to it)
-            const uint64_t dQ = sdesc_sw128(smem_u32(sQ + qs * Tile::q_bytes), 16, 1024);
-            const uint64_t dK = sdesc_sw128(smem_u32(sKV + st * Tile::kv_bytes), 16, HALVES * 1024);
-  #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks)
-              umma_bf16(tmem + s * 128, dQ + ((ks >> 2) * 16384 + (ks & 3) * 32) / 16,
-                        dK + ((ks >> 2) * 1024 + (ks & 3) * 32) / 16, idS, ks > 0 ? 1u : 0u);
-            umma_commit(&bar_s[s]);
-            if (!pair || s == 1) umma_commit(&bar_empty[st]);
-            if (pair ? u + 2 >= steps : u + 1 == steps) umma_commit(&bar_q_empty[qs]);
+      // ---------------- MMA issuer: one thread ----------------
+      if (elect_one()) {
+        constexpr uint32_t idS = paged_idesc<T>(128, PA_BN, 0, 0);
+        constexpr uint32_t idO = paged_idesc<T>(128, D, 0, 1);
+        // (a descriptor's low bits are the address / 16, so offsets are added to it)
+        const uint64_t dKV = sdesc_sw128(smem_u32(sKV), 16, HALVES * 1024);   // K-major
+        const uint64_t dVm = sdesc_sw128(smem_u32(sKV), 1024, HALVES * 1024);  // MN-major
+        // V as the A operand: D 64 has no second block of 64 columns, rows 64..127 repeat the first
+        const uint64_t dVa = sdesc_sw128(smem_u32(sKV), HALVES == 2 ? 1024 : 0, HALVES * 1024);
+        const uint64_t dQ0 = sdesc_sw128(smem_u32(sQ), 16, 1024), dP0 = sdesc_sw128(smem_u32(sQ + PA_PT), 16, 1024);
+        uint32_t npiece = 0, nfix = 0, nq = 0;  // pieces, blocks with cleared V rows, query tiles so far
+        uint32_t st0 = 0, ph0 = 0;              // ring position of the piece's first load
+        uint32_t np[2] = {0, 0}, np2[2] = {0, 0};
+        auto advance = [](uint32_t& st, uint32_t& ph, int by) {
+          st += by;
+          if (st >= ST) {
+            st -= ST;
+            ph ^= 1;
           }
-          __syncwarp();
         };
-        auto issue_pv = [&](int u) {
-          const int s = u & 1;
-          const int k = pair ? u >> 1 : u;
-          const uint32_t c = ld0 + (pair ? 2 * k + 1 : (k + 1 == nblk ? 2 * nblk - 1 : 2 * k + 2)), st = c % ST;
-          const int valid = min(PA_BN, piece.limit - (piece.j0 + k) * PA_BN);  // visible keys of the block
-          const int ksteps = (valid + 15) >> 4;
-          uint8_t* sV = sKV + st * Tile::kv_bytes;
-          if (ok && (!pair || s == 0)) {
-            ok = mbar_wait(&bar_full[st], (c / ST) & 1);
-            if (ok && (valid & 15) != 0) {
-              // rows up to the next multiple of 16 that no query sees
-              for (int i = lane; i < (ksteps * 16 - valid) * HALVES * 8; i += 32) {
-                const int r = valid + i / (HALVES * 8), ch = i % (HALVES * 8);
-                *reinterpret_cast<uint4*>(sV + (r >> 3) * (HALVES * 1024) + (ch >> 3) * 1024 + (r & 7) * 128 +
-                                          (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+        PagedPiece piece;
+        bool ok = true;
+        for (;;) {
+          const int ip = npiece % PA_PIECES;
+          if (!mbar_wait(&sh.bar_piece[ip], (npiece / PA_PIECES) & 1)) break;
+          piece = sh.piece[ip];
+          mbar_arrive(&sh.bar_taken[ip]);
+          ++npiece;
+          const int nblk = piece.nblk;
+          if (nblk <= 0) break;
+          const bool pair = piece.tokens > p.TQ, few = piece.tokens <= p.TQ_few;
+          const int steps = pair ? 2 * nblk : nblk;
+          const int n_few = paged_few_cols(piece.tokens * p.G);
+          const uint32_t idSt = paged_idesc<T>(128, n_few, 0, 0), idOt = paged_idesc<T>(128, n_few, 1, 1);
+          // visible keys of the last block: products stop at the next multiple of 16
+          const int last = min(PA_BN, piece.limit - (piece.j0 + nblk - 1) * PA_BN);
+          uint32_t kst = st0, kph = ph0, vst = st0, vph = ph0;
+          advance(vst, vph, pair || nblk == 1 ? 1 : 2);
+          // S runs two steps ahead: S0 S1 PV0 S2 PV1 S3 ...
+#pragma unroll 1
+          for (int v = 0; ok && v < steps + 2; ++v) {
+            const int s = v & 1;
+            const uint32_t tS = tmem + s * 128, tO = tmem + T_O + s * 128;
+            if (v >= 2) {
+              const int u = v - 2, k = pair ? u >> 1 : u;
+              const bool tail = k + 1 == nblk && last < PA_BN;
+              const int ksteps = tail ? (last + 15) >> 4 : PA_BN / 16;
+              const uint32_t off = vst * (Tile::kv_bytes / 16);
+              if (!pair || s == 0) {
+                ok = mbar_wait(&sh.bar_full[vst], vph);
+                if (ok && tail && (last & 15) != 0) {
+                  mbar_arrive(&sh.bar_tail);
+                  ok = mbar_wait(&sh.bar_fix, nfix++ & 1);
+                }
               }
-              fence_async_smem();
+              ok = ok && mbar_wait(&sh.bar_p[s], np[s]++ & 1);
+              if (!ok) break;
+              tc_fence_after();
+              if (few) {
+                const uint64_t dP = dP0 + s * (PA_SLOT / 16);
+                umma_bf16(tO, dVa + off, dP, idOt, u >= 2 ? 1u : 0u);
+                if (!tail) {
+#pragma unroll
+                  for (int ks = 1; ks < PA_BN / 16; ++ks)
+                    umma_bf16(tO, dVa + off + ks * (HALVES * 2048 / 16), dP + ks * (2048 / 16), idOt, 1u);
+                } else {
+#pragma unroll 1
+                  for (int ks = 1; ks < ksteps; ++ks)
+                    umma_bf16(tO, dVa + off + ks * (HALVES * 2048 / 16), dP + ks * (2048 / 16), idOt, 1u);
+                }
+              } else {
+                // the first half of P, then (its own barrier) the second
+                umma_bf16_ts(tO, tS, dVm + off, idO, u >= 2 ? 1u : 0u);
+                if (!tail) {
+#pragma unroll
+                  for (int ks = 1; ks < PA_BN / 32; ++ks)
+                    umma_bf16_ts(tO, tS + ks * 8, dVm + off + ks * (HALVES * 2048 / 16), idO, 1u);
+                } else {
+#pragma unroll 1
+                  for (int ks = 1; ks < min(ksteps, PA_BN / 32); ++ks)
+                    umma_bf16_ts(tO, tS + ks * 8, dVm + off + ks * (HALVES * 2048 / 16), idO, 1u);
+                }
+                ok = mbar_wait(&sh.bar_p2[s], np2[s]++ & 1);
+                if (!ok) break;
+                tc_fence_after();
+                if (!tail) {
+#pragma unroll
+                  for (int ks = PA_BN / 32; ks < PA_BN / 16; ++ks)
+                    umma_bf16_ts(tO, tS + ks * 8, dVm + off + ks * (HALVES * 2048 / 16), idO, 1u);
+                } else {
+#pragma unroll 1
+                  for (int ks = PA_BN / 32; ks < ksteps; ++ks)
+                    umma_bf16_ts(tO, tS + ks * 8, dVm + off + ks * (HALVES * 2048 / 16), idO, 1u);
+                }
+              }
+              if (!pair || s == 1) {
+                umma_commit(&sh.bar_empty[vst]);
+                advance(vst, vph, pair || k + 2 < nblk ? 2 : 1);
+              }
+              if (u + 2 >= steps) umma_commit(&sh.bar_o[s]);
+            }
+            if (v < steps) {
+              const uint32_t qi = nq + (pair ? s : 0), qs = qi & 1;
+              if (!pair || s == 0) ok = mbar_wait(&sh.bar_full[kst], kph);
+              if (v == 0 || (pair && v == 1)) ok = ok && mbar_wait(&sh.bar_q_full[qs], (qi >> 1) & 1);
+              if (!ok) break;
+              tc_fence_after();
+              const uint64_t dK = dKV + kst * (Tile::kv_bytes / 16), dQ = dQ0 + qs * (PA_SLOT / 16);
+              if (few) {
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks)
+                  umma_bf16(tS, dK + ((ks >> 2) * 1024 + (ks & 3) * 32) / 16,
+                            dQ + ((ks >> 2) * 8192 + (ks & 3) * 32) / 16, idSt, ks > 0 ? 1u : 0u);
+              } else {
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks)
+                  umma_bf16(tS, dQ + ((ks >> 2) * 16384 + (ks & 3) * 32) / 16,
+                            dK + ((ks >> 2) * 1024 + (ks & 3) * 32) / 16, idS, ks > 0 ? 1u : 0u);
+              }
+              umma_commit(&sh.bar_s[s]);
+              if (!pair || s == 1) {
+                umma_commit(&sh.bar_empty[kst]);
+                advance(kst, kph, pair || v > 0 ? 2 : 1);
+              }
+              if (!few && (pair ? v + 2 >= steps : v + 1 == steps)) umma_commit(&sh.bar_q_empty[qs]);
             }
           }
-          if (ok) ok = mbar_wait(&bar_p[s], np[s] & 1);
-          ++np[s];
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) return;
-          tc_fence_after();
-          if (lane == 0) {
-            const uint64_t dV = sdesc_sw128(smem_u32(sV), 1024, HALVES * 1024);
-  #pragma unroll
-            for (int ks = 0; ks < PA_BN / 16; ++ks)
-              if (ks < ksteps)
-                umma_bf16_ts(tmem + T_O + s * 128, tmem + s * 128 + ks * 8, dV + ks * (HALVES * 2048 / 16), idO,
-                             (u >= 2 || ks > 0) ? 1u : 0u);
-            if (!pair || s == 1) umma_commit(&bar_empty[st]);
-            if (u + 2 >= steps) umma_commit(&bar_o[s]);
-          }
-          __syncwarp();
-        };
-        // S runs two steps ahead: S0 S1 PV0 S2 PV1 S3 ...
-  #pragma unroll 1
-        for (int v = 0; ok && v < steps + 2; ++v) {
-          if (v >= 2) issue_pv(v - 2);
-          if (ok && v < steps) issue_s(v);
+          if (!ok) break;
+          nq += pair ? 2 : 1;
+          const int loads = (2 * nblk) % (2 * ST);  // two turns of the ring keep the parity
+          for (int i = 0; i < loads; i += 2) advance(st0, ph0, 2);
         }
-        ld0 += 2 * nblk;
-        q0 += pair ? 2 : 1;
-      }
-      // nothing may be in flight when the CTA gives back its TMEM
-      if (lane == 0) {
-        umma_commit(&bar_end);
-        mbar_wait(&bar_end, 0);
+        // nothing may be in flight when the CTA gives back its TMEM
+        umma_commit(&sh.bar_end);
+        mbar_wait(&sh.bar_end, 0);
       }
       __syncwarp();
+    } else if (warp == 11) {
+      // ---------------- clears the V rows of a tail that no query sees ----------------
+      // (up to the multiple of 16 at which the products stop)
+      uint32_t npiece = 0, ld0 = 0, nfix = 0;
+      PagedPiece piece;
+      while (next_piece(npiece, piece)) {
+        const int nblk = piece.nblk, last = piece.limit - (piece.j0 + nblk - 1) * PA_BN;
+        ld0 += 2 * nblk;
+        if (last >= PA_BN || (last & 15) == 0) continue;
+        if (!__all_sync(0xffffffffu, mbar_wait(&sh.bar_tail, nfix++ & 1))) break;  // the MMA thread has it
+        uint8_t* sV = sKV + ((ld0 - 1) % ST) * Tile::kv_bytes;                     // the piece's last load
+        for (int i = lane; i < (16 - (last & 15)) * HALVES * 8; i += 32) {
+          const int r = last + i / (HALVES * 8), ch = i % (HALVES * 8);
+          *reinterpret_cast<uint4*>(sV + (r >> 3) * (HALVES * 1024) + (ch >> 3) * 1024 + (r & 7) * 128 +
+                                    (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.bar_fix);
+      }
     } else if (warp == 10) {
       // ---------------- scheduler: the pieces of this CTA's share ----------------
+      // Costs of all requests first: chunks of 32, a request per lane, four
+      // chunks' lengths in flight at a time.
+      auto chunk_cost = [&](int n, int kv) -> long long {
+        const int items = (n + 2 * p.TQ - 1) / (2 * p.TQ);
+        int t0, nt, limit, nb, w;
+        long long cost = 0;
+        if (items == 1) {
+          paged_item(p, n, kv, 0, t0, nt, limit, nb, w);
+          cost = static_cast<long long>(nb) * w;
+        }
+        // a request of several items is summed by the whole warp
+        for (uint32_t many = __ballot_sync(0xffffffffu, items > 1); many != 0; many &= many - 1) {
+          const int src = __ffs(many) - 1;
+          const int n_ = __shfl_sync(0xffffffffu, n, src), kv_ = __shfl_sync(0xffffffffu, kv, src);
+          const int items_ = __shfl_sync(0xffffffffu, items, src);
+          long long sum = 0;
+          for (int i = lane; i < items_; i += 32) {
+            paged_item(p, n_, kv_, i, t0, nt, limit, nb, w);
+            sum += static_cast<long long>(nb) * w;
+          }
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          if (lane == src) cost = sum;
+        }
+        return cost * p.Hkv;
+      };
+      constexpr int AHEAD = 4;
+      auto lengths = [&](int b0, int* n, int* kv) {
+        int q0[AHEAD], q1[AHEAD];
+#pragma unroll
+        for (int c = 0; c < AHEAD; ++c) {
+          const int b = b0 + 32 * c + lane;
+          q0[c] = b < p.B ? __ldg(p.cu_q + b) : 0;
+          q1[c] = b < p.B ? __ldg(p.cu_q + b + 1) : 0;
+          kv[c] = b < p.B ? __ldg(p.kv_lens + b) : 0;
+        }
+#pragma unroll
+        for (int c = 0; c < AHEAD; ++c)
+          if (!paged_request(p, q0[c], q1[c], kv[c], n[c]) && cta == 0) std_set_error(STD_DEVERR_LENGTH);
+      };
+      long long total = 0;
+      long long cost[AHEAD];  // of the last four chunks seen: all of them when B <= 128
+      for (int b0 = 0; b0 < p.B; b0 += 32 * AHEAD) {
+        int n[AHEAD], kv[AHEAD];
+        lengths(b0, n, kv);
+#pragma unroll
+        for (int c = 0; c < AHEAD; ++c) {
+          cost[c] = b0 + 32 * c < p.B ? chunk_cost(n[c], kv[c]) : 0;
+          total += cost[c];
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+      // equal shares, of two blocks at least (a single's streams take one each)
+      const long long share = max((total + PA_CTAS - 1) / PA_CTAS, static_cast<long long>(2 * PA_W1));
+      const long long x0 = share * cta;
       PagedWalk walk;
-      walk.b = s_b;
       walk.rem = 0;
-      if (s_b >= 0) {
+      if (x0 < total) {
         walk.rem = min(share, total - x0);
+        long long run = 0, off = 0;
+        walk.b = -1;
+        for (int b0 = 0; walk.b < 0 && b0 < p.B; b0 += 32 * AHEAD) {
+          int n[AHEAD], kv[AHEAD];
+          if (p.B > 32 * AHEAD) lengths(b0, n, kv);
+#pragma unroll
+          for (int c = 0; c < AHEAD; ++c) {
+            if (walk.b >= 0) continue;
+            const long long mine = p.B > 32 * AHEAD ? chunk_cost(n[c], kv[c]) : cost[c];
+            long long inc = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const long long u = __shfl_up_sync(0xffffffffu, inc, o);
+              if (lane >= o) inc += u;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, x0 < run + inc);
+            if (past != 0) {
+              const int src = __ffs(past) - 1;
+              walk.b = b0 + 32 * c + src;
+              off = x0 - __shfl_sync(0xffffffffu, run + inc - mine, src);
+            }
+            run += __shfl_sync(0xffffffffu, inc, 31);
+          }
+        }
+        if (walk.b < 0) walk.b = 0;  // (only if the lengths changed under the call)
         walk.request(p);
-        long long off = s_off;
+        int t0, nt, limit, nb, w;
         long long head = 0;  // cost of one KV head of this request
-        {
-          int t0, nt, limit, nb, w;
+        if (walk.items == 1) {
+          paged_item(p, walk.n, walk.kv, 0, t0, nt, limit, nb, w);
+          head = static_cast<long long>(nb) * w;
+        } else {
           for (int i = lane; i < walk.items; i += 32) {
             paged_item(p, walk.n, walk.kv, i, t0, nt, limit, nb, w);
             head += static_cast<long long>(nb) * w;
           }
-    #pragma unroll
+#pragma unroll
           for (int o = 16; o > 0; o >>= 1) head += __shfl_xor_sync(0xffffffffu, head, o);
-          walk.h = static_cast<int>(off / head);
-          off -= walk.h * head;
-          walk.i = 0;
-          for (;;) {
-            paged_item(p, walk.n, walk.kv, walk.i, t0, nt, limit, nb, w);
-            const long long cost = static_cast<long long>(nb) * w;
-            if (off < cost) break;
-            off -= cost;
-            ++walk.i;
-          }
+        }
+        for (walk.h = 0; off >= head && walk.h + 1 < p.Hkv; ++walk.h) off -= head;
+        for (walk.i = 0; walk.i + 1 < walk.items; ++walk.i) {
+          paged_item(p, walk.n, walk.kv, walk.i, t0, nt, limit, nb, w);
+          const long long c = static_cast<long long>(nb) * w;
+          if (off < c) break;
+          off -= c;
         }
         walk.skip = off;
       }
@@ -694,7 +1148,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       for (uint32_t n = 0; more; ++n) {
         more = walk.next(p);
         const int i = n % PA_PIECES;
-        if (n >= PA_PIECES && !__all_sync(0xffffffffu, mbar_wait(&bar_taken[i], ((n / PA_PIECES) - 1) & 1))) break;
+        if (n >= PA_PIECES && !__all_sync(0xffffffffu, mbar_wait(&sh.bar_taken[i], ((n / PA_PIECES) - 1) & 1))) break;
         if (lane == 0) {
           PagedPiece piece = {walk.b, walk.h, walk.q0 + walk.t0, walk.nt, walk.limit, 0, walk.j0, 0, -1};
           if (more) {
@@ -702,8 +1156,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             piece.nblk = walk.j1 - walk.j0;
             if (walk.j0 > 0 || walk.j1 < walk.nb) piece.slot = 2 * cta + (walk.j0 == 0 ? 1 : 0);
           }
-          s_piece[i] = piece;
-          mbar_arrive(&bar_piece[i]);
+          sh.piece[i] = piece;
+          mbar_arrive(&sh.bar_piece[i]);
         }
         __syncwarp();
         if (more && walk.j0 == 0 && walk.j1 < walk.nb) {
@@ -824,12 +1278,12 @@ extern "C" size_t std_paged_attn_workspace_bytes(int D) {
 }
 
 template <typename T, int D>
-static int paged_attn_launch(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv,
+static int paged_attn_launch(const CUtensorMap& tq, const CUtensorMap& tqf, const CUtensorMap& tk, const CUtensorMap& tv,
                              const stdb::PagedAttnParams& p, cudaStream_t s) {
   static SmemGrant grant;
   if (ensure_smem(stdb::paged_attn_kernel<T, D>, grant, stdb::PagedTile<D>::smem) != 0) return 3;
   if (launch_pdl(stdb::paged_attn_kernel<T, D>, dim3(stdb::PA_CTAS), dim3(stdb::PA_THREADS), stdb::PagedTile<D>::smem,
-                 s, tq, tk, tv, p) != cudaSuccess)
+                 s, tq, tqf, tk, tv, p) != cudaSuccess)
     return 4;
   // rows that an item can have: all of a pair's 256, or those of all the tokens there are
   const int rows = p.T > p.TQ ? 256 : p.T * p.G;
@@ -857,8 +1311,8 @@ extern "C" int std_paged_attn(const void* q, const void* k_pages, const void* v_
     return 1;
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out)) return 1;
   if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < std_paged_attn_workspace_bytes(D)) return 5;
-  const int G = Hq / Hkv, TQ = 128 / G;
-  CUtensorMap tq, tk, tv;
+  const int G = Hq / Hkv, TQ = 128 / G, TQ_few = stdb::PA_FEW / G;
+  CUtensorMap tq, tqf, tk, tv;
   {
     const uint64_t e = 2, row = static_cast<uint64_t>(D) * e;
     const uint64_t qd[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(G), static_cast<uint64_t>(Hkv),
@@ -866,6 +1320,10 @@ extern "C" int std_paged_attn(const void* q, const void* k_pages, const void* v_
     const uint64_t qs[3] = {row, row * G, row * Hq};
     const uint32_t qb[4] = {64, static_cast<uint32_t>(G), 1, static_cast<uint32_t>(TQ)};
     int rc = paged_tmap_4d(&tq, is_fp16, q, qd, qs, qb);
+    if (rc != 0) return rc;
+    // (heads in groups of more than 64 have no few-row items: the map is not used)
+    const uint32_t qfb[4] = {64, static_cast<uint32_t>(G), 1, static_cast<uint32_t>(TQ_few > 0 ? TQ_few : 1)};
+    rc = paged_tmap_4d(&tqf, is_fp16, q, qd, qs, qfb);
     if (rc != 0) return rc;
     const uint64_t kd[4] = {64, 8, static_cast<uint64_t>(D / 64),
                             static_cast<uint64_t>(num_pages) * Hkv * (page_size / 8)};
@@ -883,12 +1341,14 @@ extern "C" int std_paged_attn(const void* q, const void* k_pages, const void* v_
   p.T = T;
   p.B = B;
   p.width = max_blocks;
-  p.page = page_size;
+  p.page_log2 = 0;
+  while ((1 << p.page_log2) < page_size) ++p.page_log2;
   p.num_pages = num_pages;
   p.Hq = Hq;
   p.Hkv = Hkv;
   p.G = G;
   p.TQ = TQ;
+  p.TQ_few = TQ_few;
   p.causal = causal != 0 ? 1 : 0;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.out = out;
@@ -899,8 +1359,8 @@ extern "C" int std_paged_attn(const void* q, const void* k_pages, const void* v_
   p.splits = reinterpret_cast<stdb::PagedSplit*>(ws + paged_ws_o_bytes(D) + paged_ws_ml_bytes());
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (D == 128)
-    return is_fp16 ? paged_attn_launch<__half, 128>(tq, tk, tv, p, s)
-                   : paged_attn_launch<__nv_bfloat16, 128>(tq, tk, tv, p, s);
-  return is_fp16 ? paged_attn_launch<__half, 64>(tq, tk, tv, p, s)
-                 : paged_attn_launch<__nv_bfloat16, 64>(tq, tk, tv, p, s);
+    return is_fp16 ? paged_attn_launch<__half, 128>(tq, tqf, tk, tv, p, s)
+                   : paged_attn_launch<__nv_bfloat16, 128>(tq, tqf, tk, tv, p, s);
+  return is_fp16 ? paged_attn_launch<__half, 64>(tq, tqf, tk, tv, p, s)
+                 : paged_attn_launch<__nv_bfloat16, 64>(tq, tqf, tk, tv, p, s);
 }

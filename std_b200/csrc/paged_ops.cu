@@ -247,6 +247,12 @@ struct PairOf<__half> {
   static STD_DEV __half2 make(float a, float b) { return __floats2half2_rn(a, b); }
 };
 template <typename T>
+STD_DEV T to_type(float v);
+template <>
+STD_DEV __nv_bfloat16 to_type<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+STD_DEV __half to_type<__half>(float v) { return __float2half_rn(v); }
+template <typename T>
 STD_DEV uint32_t pack_pair(float a, float b) {
   const typename PairOf<T>::type v = PairOf<T>::make(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);

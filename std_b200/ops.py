@@ -18,7 +18,8 @@ _WS: Dict[Tuple[str, int], torch.Tensor] = {}
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # the raw handle of torch.cuda.current_stream(), without building a Stream object (3 us a call)
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _p(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -381,39 +382,39 @@ def argmax_rows(logits: torch.Tensor, out: torch.Tensor, n: int = 1, out_stride:
 _PAGED_DTYPES = (torch.bfloat16, torch.float16)
 
 
-def _paged_tensor(t: torch.Tensor, name: str, shape: Tuple[int, ...], dtype: torch.dtype, device: torch.device) -> None:
-    """A contiguous tensor of this shape and type on the call's device."""
-    if not isinstance(t, torch.Tensor):
-        raise RuntimeError(f"{name} must be a tensor")
-    _check(t, dtype, name)
-    if t.device != device:
-        raise RuntimeError(f"{name} is on {t.device}, the call's other tensors on {device}")
-    if tuple(t.shape) != tuple(shape):
+def _paged_check(dtype: torch.dtype, device: int, *tensors) -> None:
+    """Each (tensor, name, shape): contiguous, of this shape and type, on the
+    call's device.  (These checks are most of a small call's time: one pass.)"""
+    for t, name, shape in tensors:
+        if t.dtype is dtype and t.get_device() == device and t.shape == shape and t.is_contiguous():
+            continue
+        _check(t, dtype, name)
+        if t.get_device() != device:
+            raise RuntimeError(f"{name} is on {t.device}, the call's other tensors on cuda:{device}")
         raise ValueError(f"{name} must have shape {list(shape)}, got {list(t.shape)}")
 
 
-def _paged_device(t: torch.Tensor, name: str) -> torch.device:
+def _paged_device(t: torch.Tensor, name: str) -> int:
     """The call's device: kernels run on the current device's stream, so it
     has to be that one."""
-    if not t.is_cuda:
+    device = t.get_device()
+    if device < 0:
         raise RuntimeError(f"{name} must be a CUDA tensor (no CPU path)")
-    if t.device.index != torch.cuda.current_device():
+    if device != torch.cuda.current_device():
         raise RuntimeError(f"{name} is on {t.device}, but cuda:{torch.cuda.current_device()} is the current device")
-    return t.device
+    return device
 
 
-def _paged_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtype,
-                device: torch.device) -> Tuple[int, int, int, int]:
+def _paged_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtype, device: int):
     if k_pages.dim() != 4:
         raise ValueError("k_pages must be [num_pages, Hkv, page_size, D]")
-    _paged_tensor(k_pages, "k_pages", k_pages.shape, dtype, device)
-    _paged_tensor(v_pages, "v_pages", k_pages.shape, dtype, device)
-    num_pages, Hkv, page, D = k_pages.shape
-    if page not in (16, 32, 64, 128, 256):
-        raise ValueError(f"page_size must be 16, 32, 64, 128 or 256, got {page}")
-    if D not in (64, 128):
-        raise ValueError(f"head dim must be 64 or 128, got {D}")
-    return num_pages, Hkv, page, D
+    shape = k_pages.shape
+    _paged_check(dtype, device, (k_pages, "k_pages", shape), (v_pages, "v_pages", shape))
+    if shape[2] not in (16, 32, 64, 128, 256):
+        raise ValueError(f"page_size must be 16, 32, 64, 128 or 256, got {shape[2]}")
+    if shape[3] not in (64, 128):
+        raise ValueError(f"head dim must be 64 or 128, got {shape[3]}")
+    return shape
 
 
 def paged_update(past_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, n_blocks: torch.Tensor,
@@ -435,22 +436,24 @@ def paged_update(past_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
         raise ValueError("paged_update needs at least one request")
     if block_table.dim() != 2:
         raise ValueError("block_table must be [B, max_blocks]")
-    width, num_pages = block_table.shape[1], free_pages.numel()
-    if not 0 <= int(max_tokens) < 2 ** 31:
+    width, num_pages, max_tokens = block_table.shape[1], free_pages.numel(), int(max_tokens)
+    if not 0 <= max_tokens < 2 ** 31:
         raise ValueError("max_tokens must be a non-negative int32")
-    for t, name, shape in ((past_lens, "past_lens", (B,)), (new_lens, "new_lens", (B,)),
-                           (block_table, "block_table", (B, width)), (n_blocks, "n_blocks", (B,)),
-                           (free_pages, "free_pages", (num_pages,)), (n_free, "n_free", (1,))):
-        _paged_tensor(t, name, shape, i32, device)
+    _paged_check(i32, device, (past_lens, "past_lens", (B,)), (new_lens, "new_lens", (B,)),
+                 (block_table, "block_table", (B, width)), (n_blocks, "n_blocks", (B,)),
+                 (free_pages, "free_pages", (num_pages,)), (n_free, "n_free", (1,)))
     if out is None:
-        out = tuple(torch.empty(n, dtype=i32, device=device) for n in (B + 1, B, max_tokens, max_tokens, B))
-    cu_q, kv_lens, slots, positions, admitted = out
-    for t, name, n in ((cu_q, "cu_q", B + 1), (kv_lens, "kv_lens", B), (slots, "slots", max_tokens),
-                       (positions, "positions", max_tokens), (admitted, "admitted", B)):
-        _paged_tensor(t, name, (n,), i32, device)
+        sizes = (B + 1, B, B, max_tokens, max_tokens)
+        cu_q, kv_lens, admitted, slots, positions = torch.empty(
+            sum(sizes), dtype=i32, device=past_lens.device).split_with_sizes(sizes)
+    else:
+        cu_q, kv_lens, slots, positions, admitted = out
+        _paged_check(i32, device, (cu_q, "cu_q", (B + 1,)), (kv_lens, "kv_lens", (B,)),
+                     (slots, "slots", (max_tokens,)), (positions, "positions", (max_tokens,)),
+                     (admitted, "admitted", (B,)))
     _lib.call("std_paged_update", past_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
               n_blocks.data_ptr(), free_pages.data_ptr(), n_free.data_ptr(), B, width, int(page_size), num_pages,
-              int(max_tokens), cu_q.data_ptr(), kv_lens.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+              max_tokens, cu_q.data_ptr(), kv_lens.data_ptr(), slots.data_ptr(), positions.data_ptr(),
               admitted.data_ptr(), _stream())
     return cu_q, kv_lens, slots, positions, admitted
 
@@ -470,11 +473,9 @@ def paged_rope_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.T
     num_pages, Hkv, page, D = _paged_pool(k_pages, v_pages, dtype, device)
     T, Hq = q_out.shape[:2]
     max_pos = cos_t.shape[0]
-    for t, name, shape in ((q_out, "q_out", (T, Hq, D)), (qkv, "qkv", (T, (Hq + 2 * Hkv) * D)),
-                           (cos_t, "cos_t", (max_pos, D // 2)), (sin_t, "sin_t", (max_pos, D // 2))):
-        _paged_tensor(t, name, shape, dtype, device)
-    for t, name in ((positions, "positions"), (slots, "slots")):
-        _paged_tensor(t, name, (T,), torch.int32, device)
+    _paged_check(dtype, device, (q_out, "q_out", (T, Hq, D)), (qkv, "qkv", (T, (Hq + 2 * Hkv) * D)),
+                 (cos_t, "cos_t", (max_pos, D // 2)), (sin_t, "sin_t", (max_pos, D // 2)))
+    _paged_check(torch.int32, device, (positions, "positions", (T,)), (slots, "slots", (T,)))
     _lib.call("std_paged_rope_append", qkv.data_ptr(), T, Hq, Hkv, D, 1 if dtype == torch.float16 else 0,
               positions.data_ptr(), slots.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), max_pos, q_out.data_ptr(),
               k_pages.data_ptr(), v_pages.data_ptr(), num_pages, page, _stream())
@@ -502,24 +503,23 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     T, Hq, D = q.shape
     num_pages, Hkv, page, _ = _paged_pool(k_pages, v_pages, dtype, device)
     B, width = block_table.shape
-    _paged_tensor(q, "q", (T, Hq, k_pages.shape[3]), dtype, device)
+    _paged_check(dtype, device, (q, "q", (T, Hq, k_pages.shape[3])))
     if Hkv < 1 or Hq % Hkv != 0 or not 1 <= Hq // Hkv <= 128:
         raise ValueError(f"query heads ({Hq}) must be a multiple of key heads ({Hkv}), at most 128 times as many")
-    for t, name, shape in ((block_table, "block_table", (B, width)), (cu_q, "cu_q", (B + 1,)),
-                           (kv_lens, "kv_lens", (B,))):
-        _paged_tensor(t, name, shape, torch.int32, device)
+    _paged_check(torch.int32, device, (block_table, "block_table", (B, width)), (cu_q, "cu_q", (B + 1,)),
+                 (kv_lens, "kv_lens", (B,)))
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 0.0 < scale < 3e38:
         raise ValueError(f"scale must be positive and finite, got {scale}")
     if out is None:
         out = torch.empty_like(q)
     else:
-        _paged_tensor(out, "out", (T, Hq, D), dtype, device)
+        _paged_check(dtype, device, (out, "out", (T, Hq, D)))
     if lse is not None:
-        _paged_tensor(lse, "lse", (T, Hq), torch.float32, device)
+        _paged_check(torch.float32, device, (lse, "lse", (T, Hq)))
     # Of this call alone: the caching allocator hands it out in stream order, and
     # under capture from the graph's own pool, so no two calls or graphs share it.
-    ws = torch.empty(_lib.query("std_paged_attn_workspace_bytes", D), dtype=torch.uint8, device=device)
+    ws = torch.empty(_lib.query("std_paged_attn_workspace_bytes", D), dtype=torch.uint8, device=q.device)
     _lib.call("std_paged_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
               cu_q.data_ptr(), kv_lens.data_ptr(), T, B, Hq, Hkv, D, 1 if dtype == torch.float16 else 0, num_pages,
               page, width, 1 if causal else 0, scale, out.data_ptr(), _p(lse), ws.data_ptr(), ws.numel(), _stream())
