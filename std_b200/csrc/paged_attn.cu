@@ -21,7 +21,7 @@
 //
 // Few rows.  A single item of at most 64 rows (decoding: G rows) is computed
 // transposed, keys on the 128 MMA rows and the query rows on N:
-//   S^T = K Q^T    M=128 (keys) N=16, 32 or 64, both operands in shared memory
+//   S^T = K Q^T    M=128 (keys) N=16 or 64, both operands in shared memory
 //   O^T += V^T P^T M=128 (head dims), A = V MN-major, B = P^T in shared memory
 // A softmax thread then owns one key and N rows, so a block costs N exponentials
 // a thread on all 128 threads instead of 128 on the few threads that have a row,
@@ -54,7 +54,9 @@ constexpr int PA_THREADS = 384;  // 2 softmax warpgroups; TMA, MMA, scheduler an
 constexpr int PA_REGS_SOFTMAX = 208, PA_REGS_OTHER = 88;
 constexpr int PA_BN = 128;       // keys per block
 constexpr float PA_RESCALE = 8.0f;  // log2 units
-constexpr int PA_W1 = 2, PA_W2 = 3;  // cost of a block in a single and in a pair
+// Cost of a block in a single and in a pair; an item costs PA_OVER blocks more
+// (its queries, first keys and output).
+constexpr int PA_W1 = 2, PA_W2 = 3, PA_OVER = 2;
 
 // Shared memory: two query slots and a ring of K/V blocks.  A slot holds a
 // 128-row Q tile (halves of 64 columns, 16 KB apart), or, for few rows, a 64-row
@@ -68,7 +70,6 @@ struct PagedTile {
   static constexpr uint32_t smem = 2 * PA_SLOT + stages * kv_bytes + 1024;
 };
 constexpr int PA_FEW = 64;  // most rows of an item that is computed transposed
-constexpr float PA_LOW = -1e30f;  // few rows: m before the first key
 constexpr int PA_POLY = 4;  // every 4th pair of exponentials on the FMA pipe
 
 // What a CTA leaves for the merge about the item that its share ends inside.
@@ -86,6 +87,8 @@ struct PagedAttnParams {
   int T, B, width, page_log2, num_pages, Hq, Hkv, G, TQ, TQ_few, causal;  // TQ_few = floor(64 / G)
   float scale_log2;
   void* out;   // [T, Hq, D]
+  int out_32b;    // out is 32-byte aligned
+  int unit_log2;  // of the costs
   float* lse;  // [T, Hq], may be null
   float* ws_o;        // [2 * PA_CTAS][256][D]
   float2* ws_ml;      // [2 * PA_CTAS][256]
@@ -101,7 +104,18 @@ STD_DEV bool paged_request(const PagedAttnParams& p, int q0, int q1, int& kv, in
   kv = kv < 0 ? 0 : (kv > room ? room : kv);
   return fit;
 }
-// Item i of a request: its tokens, the last key that any of them sees (+1).
+STD_DEV int paged_kv(const PagedAttnParams& p, int b) { return min(max(__ldg(p.kv_lens + b), 0), p.width << p.page_log2); }
+// Inclusive sums over the warp's lanes.
+STD_DEV int warp_scan(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+// Item i of a request: its tokens, the last key that any of them sees (+1),
+// its blocks and what one costs.
 STD_DEV void paged_item(const PagedAttnParams& p, int n, int kv, int i, int& t0, int& nt, int& limit, int& nb, int& w) {
   t0 = i * 2 * p.TQ;
   nt = min(2 * p.TQ, n - t0);
@@ -109,8 +123,17 @@ STD_DEV void paged_item(const PagedAttnParams& p, int n, int kv, int i, int& t0,
   nb = max(1, (limit + PA_BN - 1) / PA_BN);
   w = nt > p.TQ ? PA_W2 : PA_W1;
 }
-STD_DEV int paged_ceil_w(long long x, int w) {
-  return static_cast<int>(w == PA_W1 ? (x + PA_W1 - 1) / PA_W1 : (x + PA_W2 - 1) / PA_W2);
+// Costs fit 32 bits: the host picks the unit, 2^unit_log2 (1 unless the lengths
+// that the tensors allow are extreme).
+STD_DEV int paged_item_cost(const PagedAttnParams& p, int n, int kv, int i) {
+  int t0, nt, limit, nb, w;
+  paged_item(p, n, kv, i, t0, nt, limit, nb, w);
+  return ((nb + PA_OVER) * w + (1 << p.unit_log2) - 1) >> p.unit_log2;
+}
+// The first block at or after cost x of an item: block j lies at (j + PA_OVER) w.
+STD_DEV int paged_cut(const PagedAttnParams& p, int x, int w) {
+  x <<= p.unit_log2;
+  return max(0, (w == PA_W1 ? (x + PA_W1 - 1) / PA_W1 : (x + PA_W2 - 1) / PA_W2) - PA_OVER);
 }
 
 // A piece as the other warps see it: nblk blocks from block j0 of one item.
@@ -129,11 +152,11 @@ constexpr int PA_PIECES = 4;  // ring of pieces in shared memory
 struct PagedWalk {
   int b, h, i;         // current item
   int q0, n, kv, items;
-  long long skip;      // cost of the item that earlier CTAs did
-  long long rem;       // cost left in this CTA's share
+  int skip;            // cost of the item that earlier CTAs did
+  int rem;             // cost left in this CTA's share
   // the current piece
   int t0, nt, limit, nb, w, j0, j1;
-  long long cut;       // cost of the item up to the end of this piece
+  int cut;             // cost of the item up to the end of this piece
 
   STD_DEV void request(const PagedAttnParams& p) {
     q0 = __ldg(p.cu_q + b);
@@ -153,10 +176,10 @@ struct PagedWalk {
         }
       }
       paged_item(p, n, kv, i, t0, nt, limit, nb, w);
-      const long long cost = static_cast<long long>(nb) * w;
-      const long long end = min(cost, skip + rem);
-      j0 = paged_ceil_w(skip, w);
-      j1 = paged_ceil_w(end, w);
+      const int cost = paged_item_cost(p, n, kv, i);
+      const int end = min(cost, skip + rem);
+      j0 = paged_cut(p, skip, w);
+      j1 = min(nb, paged_cut(p, end, w));
       rem -= end - skip;
       skip = 0;
       cut = end;
@@ -174,7 +197,7 @@ __host__ __device__ constexpr uint32_t paged_idesc(int M, int N, int a_mn_major,
          (std::is_same<T, __half>::value ? ~((1u << 7) | (1u << 10)) : ~0u);
 }
 // MMA columns for `rows` few rows.
-STD_DEV int paged_few_cols(int rows) { return rows <= 16 ? 16 : (rows <= 32 ? 32 : 64); }
+STD_DEV int paged_few_cols(int rows) { return rows <= 16 ? 16 : 64; }
 
 STD_DEV void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
   asm volatile(
@@ -187,14 +210,25 @@ STD_DEV void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, 
 // Static shared memory of a CTA with an ST-stage ring.
 template <int ST>
 struct PagedShared {
-  uint64_t bar_q_full[2], bar_q_empty[2];        // query slots
-  uint64_t bar_full[ST], bar_empty[ST];          // K/V ring
-  uint64_t bar_s[2], bar_p[2], bar_p2[2], bar_o[2];  // per stream: S there, P's halves there, O complete
-  uint64_t bar_join, bar_joined;                 // a single's two streams
-  uint64_t bar_group[2];                         // few rows: the four warps of a stream
-  uint64_t bar_piece[PA_PIECES], bar_taken[PA_PIECES];
-  uint64_t bar_tail, bar_fix;                    // a tail's V there, its rows cleared
-  uint64_t bar_end;
+  // mbarriers, by the arrivals that complete a phase
+  static constexpr int BARS_1 = 11 + 2 * ST + PA_PIECES, BARS_4 = BARS_1 + 8, BARS = BARS_4 + PA_PIECES;
+  union {
+    uint64_t bars[BARS];
+    struct {
+      // one
+      uint64_t bar_q_full[2], bar_q_empty[2];  // query slots
+      uint64_t bar_s[2], bar_o[2];             // per stream: S there, O complete
+      uint64_t bar_tail, bar_fix, bar_end;     // a tail's V there, its rows cleared; all MMAs done
+      uint64_t bar_full[ST], bar_empty[ST];    // K/V ring
+      uint64_t bar_piece[PA_PIECES];
+      // four (a stream's warps)
+      uint64_t bar_p[2], bar_p2[2];   // P's halves there
+      uint64_t bar_join, bar_joined;  // a single's two streams
+      uint64_t bar_group[2];          // few rows: the four warps of a stream
+      // eleven (the warps that read a piece)
+      uint64_t bar_taken[PA_PIECES];
+    };
+  };
   // A single's statistics, of one use at a time: whole tiles hand them from
   // stream 1 to stream 0, few rows keep theirs here.  A stream's warps write the
   // next piece's only after a barrier that all readers of the last have passed.
@@ -204,7 +238,7 @@ struct PagedShared {
     };
     struct {
       alignas(16) float ref[2][PA_FEW];    // m of each stream and row; the streams' weights at the join
-      alignas(16) float alpha[2][PA_FEW];  // the factor of a rescaled O
+      alignas(16) float up[2][PA_FEW];     // by how much m was raised last
     };
   };
   alignas(16) int flag[2][2][4];  // few rows: a vote per warp, by step parity
@@ -228,6 +262,12 @@ STD_DEV void tmem_st16(uint32_t taddr, const uint32_t* r) {
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+STD_DEV void tmem_ld4(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr)
+               : "memory");
 }
 template <int N>
 STD_DEV void tmem_ld_cols(uint32_t taddr, uint32_t* r) {
@@ -260,11 +300,16 @@ STD_DEV bool elect_one() {
       : "=r"(r));
   return r != 0;
 }
-// Largest value of the warp (NaN ignored).
-STD_DEV float warp_max_redux(float v) {
-  float r;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
+// 32 bytes: one store of a whole sector when the address is 32-byte aligned.
+STD_DEV void st_global_32b(void* p, const uint32_t* r, bool aligned) {
+  if (aligned)
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+  else {
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(r[0], r[1], r[2], r[3]);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(r[4], r[5], r[6], r[7]);
+  }
 }
 // Two floats in one 64-bit register, for the paired FMA and add.
 STD_DEV uint64_t f2_make(float lo, float hi) {
@@ -348,7 +393,7 @@ STD_DEV void paged_softmax_step(uint32_t tS, uint32_t tO, float sc, int nvis, fl
   if (__any_sync(0xffffffffu, need)) {
     const float alpha = need ? exp2f(m_run - m_c) : 1.0f;
     uint32_t o[32];
-#pragma unroll
+#pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
       tmem_ld32(tO + c * 32, o);
       tmem_wait_ld();
@@ -395,9 +440,36 @@ STD_DEV void paged_softmax_step(uint32_t tS, uint32_t tO, float sc, int nvis, fl
   l_run = l.x + l.y;
 }
 
+// Combines N values of each lane over the warp: halving the rows a lane keeps at
+// each step, max(1, N / 32) of them are left, rows `base` and up.
+template <int N, typename Op>
+STD_DEV int warp_reduce_rows(float* v, int lane, Op op) {
+  int base = 0;
+#pragma unroll
+  for (int o = 16, half = N / 2; o > 0; o >>= 1, half >>= 1) {
+    if (half > 0) {
+      const bool up = (lane & o) != 0;
+      base += up ? half : 0;
+#pragma unroll
+      for (int i = 0; i < (half > 0 ? half : 1); ++i) {
+        const float give = up ? v[i] : v[i + half], keep = up ? v[i + half] : v[i];
+        v[i] = op(keep, __shfl_xor_sync(0xffffffffu, give, o));
+      }
+    } else {
+      v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], o));
+    }
+  }
+  return base;
+}
+
 // A piece with few rows, for one warp of stream s (thread = key of the block,
 // N >= the piece's rows columns).  ns, no, nj, ng: phases used so far of the
-// stream's S, O, join and group barriers; bar_q_empty: its query slot's.  False when a wait ran out.
+// stream's S, O, join and group barriers; bar_q_empty: its query slot's.  False
+// when a wait ran out.
+//
+// m (sh.ref) is set to the row's maximum over the first block and raised when a
+// score passes it by 2^8, on all four warps: they vote at every block.  The keys
+// a row sees are a prefix, so a row without one in the first block has none.
 template <typename T, int D, int N, int ST>
 STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, PagedShared<ST>& sh, uint8_t* sQ,
                              uint32_t tS, uint32_t tO, int s, uint64_t* bar_q_empty, uint32_t& ns, uint32_t& no, uint32_t& nj,
@@ -418,93 +490,72 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
   float l[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) l[n] = 0.f;
-  const int all_see = p.causal ? min(piece.limit, piece.first) : piece.limit;  // keys that every row sees
+#pragma unroll 1
   for (int k = 0; k < steps; ++k, ++ns) {
     if (!__all_sync(0xffffffffu, mbar_wait(&sh.bar_s[s], ns & 1))) return false;
     tc_fence_after();
+    float y[N];
+    tmem_ld_cols<N>(tS, reinterpret_cast<uint32_t*>(y));
+    tmem_wait_ld();
+    // this key is hidden from the tokens before it, hence from rows n < hide
     const int pos = (piece.j0 + 2 * k + s) * PA_BN + key;
-    float x[N];
-    // scores, -inf where hidden and in the columns past the last row
-    auto load = [&]() {
-      tmem_ld_cols<N>(tS, reinterpret_cast<uint32_t*>(x));
-      tmem_wait_ld();
-      if (__any_sync(0xffffffffu, pos >= all_see)) {
-        int see = p.causal ? min(piece.limit, piece.first) : piece.limit, g = 0;
+    const int hide = pos >= piece.limit ? rows : (p.causal ? max(0, pos - piece.first + 1) * p.G : 0);
+    float over = -INFINITY;
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-          if (pos >= see || n >= rows) x[n] = -INFINITY;
-          if (++g == p.G) {
-            g = 0;
-            if (p.causal) see = min(piece.limit, see + 1);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-          if (n >= rows) x[n] = -INFINITY;
-      }
-    };
-    load();
-    bool fresh = k == 0;  // m has to be found (first block) or raised
+    for (int n = 0; n < N; n += 4) {
+      const float4 m = k > 0 ? *reinterpret_cast<const float4*>(&sh.ref[s][n]) : make_float4(0.f, 0.f, 0.f, 0.f);
+      y[n] = n >= hide && n < rows ? fmaf(y[n], sc, -m.x) : -INFINITY;
+      y[n + 1] = n + 1 >= hide && n + 1 < rows ? fmaf(y[n + 1], sc, -m.y) : -INFINITY;
+      y[n + 2] = n + 2 >= hide && n + 2 < rows ? fmaf(y[n + 2], sc, -m.z) : -INFINITY;
+      y[n + 3] = n + 3 >= hide && n + 3 < rows ? fmaf(y[n + 3], sc, -m.w) : -INFINITY;
+      over = fmaxf(max3(over, y[n], y[n + 1]), fmaxf(y[n + 2], y[n + 3]));
+    }
+    bool raise = k == 0;
     if (k > 0) {
-      float over = -INFINITY;
-#pragma unroll
-      for (int n = 0; n < N; n += 4) {
-        const float4 m = *reinterpret_cast<const float4*>(&sh.ref[s][n]);
-        x[n] = fmaf(x[n], sc, -m.x);
-        x[n + 1] = fmaf(x[n + 1], sc, -m.y);
-        x[n + 2] = fmaf(x[n + 2], sc, -m.z);
-        x[n + 3] = fmaf(x[n + 3], sc, -m.w);
-        over = fmaxf(max3(over, x[n], x[n + 1]), fmaxf(x[n + 2], x[n + 3]));
-      }
       const bool vote = __any_sync(0xffffffffu, over > PA_RESCALE);
       if (lane == 0) sh.flag[s][k & 1][w] = vote ? 1 : 0;
       if (!group_sync()) return false;
       const int4 f = *reinterpret_cast<const int4*>(sh.flag[s][k & 1]);
-      fresh = (f.x | f.y | f.z | f.w) != 0;
-      if (fresh) load();
+      raise = (f.x | f.y | f.z | f.w) != 0;
     }
-    if (fresh) {
+    if (raise) {
+      float v[N];
 #pragma unroll
-      for (int n = 0; n < N; ++n) {
-        const float v = warp_max_redux(x[n]);
-        if (lane == (n & 31)) red(s, w, n) = v;
-      }
+      for (int n = 0; n < N; ++n) v[n] = y[n];
+      const int base = warp_reduce_rows<N>(v, lane, [](float a, float b) { return fmaxf(a, b); });
+      red(s, w, base) = v[0];
+      if (N == 64) red(s, w, base + 1) = v[1];
       if (!group_sync()) return false;
       if (key < N) {
-        const float mx =
-            fmaxf(fmaxf(red(s, 0, key), red(s, 1, key)), fmaxf(red(s, 2, key), red(s, 3, key))) * sc;
-        const float old = k == 0 ? PA_LOW : sh.ref[s][key];
-        const float m = mx > old + PA_RESCALE ? mx : old;
-        sh.alpha[s][key] = exp2f(old - m);
-        sh.ref[s][key] = m;
+        const float mx = fmaxf(fmaxf(red(s, 0, key), red(s, 1, key)), fmaxf(red(s, 2, key), red(s, 3, key)));
+        const float up = k == 0 ? (mx > -INFINITY ? mx : 0.f) : (mx > PA_RESCALE ? mx : 0.f);
+        sh.up[s][key] = up;
+        sh.ref[s][key] = k == 0 ? up : sh.ref[s][key] + up;
       }
       if (!group_sync()) return false;
-      if (k > 0) {
-        uint32_t o[16];
 #pragma unroll
+      for (int n = 0; n < N; ++n) y[n] -= sh.up[s][n];
+      if (k > 0) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) l[n] *= ex2_approx(-sh.up[s][n]);
+        uint32_t o[16];
+#pragma unroll 1
         for (int c = 0; c < N; c += 16) {
           tmem_ld16(tO + c, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float a = sh.alpha[s][c + j];
-            l[c + j] *= a;
-            o[j] = __float_as_uint(__uint_as_float(o[j]) * a);
-          }
+          for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * ex2_approx(-sh.up[s][c + j]));
           tmem_st16(tO + c, o);
         }
         tmem_wait_st();
       }
-#pragma unroll
-      for (int n = 0; n < N; ++n) x[n] = fmaf(x[n], sc, -sh.ref[s][n]);
     }
 #pragma unroll
     for (int n = 0; n < N; n += 8) {
       float e[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        e[j] = ex2_approx(x[n + j]);
+        e[j] = ex2_approx(y[n + j]);
         l[n + j] += e[j];
       }
       *reinterpret_cast<uint4*>(row_p + (((n >> 3) ^ (key & 7)) << 4)) =
@@ -518,22 +569,7 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
   }
   if (steps > 0) {
     if (!__all_sync(0xffffffffu, mbar_wait(&sh.bar_o[s], no++ & 1))) return false;
-    // sum of l over the warp's keys, halving the rows a lane keeps at each step
-    int base = 0;
-#pragma unroll
-    for (int o = 16, half = N / 2; o > 0; o >>= 1, half >>= 1) {
-      if (half > 0) {
-        const bool up = (lane & o) != 0;
-        base += up ? half : 0;
-#pragma unroll
-        for (int i = 0; i < (half > 0 ? half : 1); ++i) {
-          const float give = up ? l[i] : l[i + half], keep = up ? l[i + half] : l[i];
-          l[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
-        }
-      } else {
-        l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
-      }
-    }
+    const int base = warp_reduce_rows<N>(l, lane, [](float a, float b) { return a + b; });
     red(s, w, base) = l[0];
     if (N == 64) red(s, w, base + 1) = l[1];
     fence_async_smem();  // (a TMA load may write here next)
@@ -553,7 +589,8 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
   if (key < N) {
     const float la = red(0, 0, key) + red(0, 1, key) + red(0, 2, key) + red(0, 3, key);
     const float lb = two ? red(1, 0, key) + red(1, 1, key) + red(1, 2, key) + red(1, 3, key) : 0.f;
-    const float ma = sh.ref[0][key], mb = two ? sh.ref[1][key] : PA_LOW, m = fmaxf(ma, mb);
+    const float ma = sh.ref[0][key], mb = sh.ref[1][key];
+    const float m = la != 0.f ? (lb != 0.f ? fmaxf(ma, mb) : ma) : mb;
     const float wa = la != 0.f ? exp2f(ma - m) : 0.f, wb = lb != 0.f ? exp2f(mb - m) : 0.f;
     const float lt = (la != 0.f ? la * wa : 0.f) + (lb != 0.f ? lb * wb : 0.f);
     const float inv = whole && lt != 0.f ? 1.f / lt : 1.f;
@@ -570,31 +607,30 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
   if (!group_sync()) return false;
   tc_fence_after();
   // thread = head dim: O^T's columns are rows
-  size_t orow = orow0;
+  T* out = static_cast<T*>(p.out) + orow0 * D + key;
+  float* part = p.ws_o + static_cast<size_t>(whole ? 0 : piece.slot) * 256 * D + key;
   int g = 0;
+#pragma unroll 1
+  for (int c = 0; c < rows; c += 4) {
+    uint32_t oa[4], ob[4] = {0, 0, 0, 0};
+    tmem_ld4(tO + c, oa);
+    if (two) tmem_ld4(tO + 128 + c, ob);
+    tmem_wait_ld();
 #pragma unroll
-  for (int c = 0; c < N; c += 16) {
-    if (c < rows) {
-      uint32_t oa[16], ob[16];
-      tmem_ld16(tO + c, oa);
-      if (two) tmem_ld16(tO + 128 + c, ob);
-      tmem_wait_ld();
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float wa = sh.ref[0][c + j], wb = sh.ref[1][c + j];
-        float v = wa != 0.f ? __uint_as_float(oa[j]) * wa : 0.f;
-        if (two) v += wb != 0.f ? __uint_as_float(ob[j]) * wb : 0.f;
-        if (c + j < rows && key < D) {
-          if (whole)
-            static_cast<T*>(p.out)[orow * D + key] = to_type<T>(v);
-          else
-            p.ws_o[(static_cast<size_t>(piece.slot) * 256 + c + j) * D + key] = v;
-        }
-        ++orow;
-        if (++g == p.G) {
-          g = 0;
-          orow += p.Hq - p.G;
-        }
+    for (int j = 0; j < 4; ++j) {
+      const float wa = sh.ref[0][c + j], wb = sh.ref[1][c + j];
+      const float v = (wa != 0.f ? __uint_as_float(oa[j]) * wa : 0.f) + (wb != 0.f ? __uint_as_float(ob[j]) * wb : 0.f);
+      if (c + j < rows && key < D) {
+        if (whole)
+          *out = to_type<T>(v);
+        else
+          *part = v;
+      }
+      out += D;
+      part += D;
+      if (++g == p.G) {
+        g = 0;
+        out += static_cast<size_t>(p.Hq - p.G) * D;
       }
     }
   }
@@ -621,34 +657,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   uint8_t* sKV = smem + 2 * PA_SLOT;  // [ST][kv_bytes]
   __shared__ PagedShared<ST> sh;
 
-  if (tid == 256) {
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&sh.bar_q_full[i], 1);
-      mbar_init(&sh.bar_q_empty[i], 1);
-      mbar_init(&sh.bar_s[i], 1);
-      mbar_init(&sh.bar_p[i], 4);
-      mbar_init(&sh.bar_o[i], 1);
-      mbar_init(&sh.bar_p2[i], 4);
-      mbar_init(&sh.bar_group[i], 4);
-    }
-    for (int i = 0; i < ST; ++i) {
-      mbar_init(&sh.bar_full[i], 1);
-      mbar_init(&sh.bar_empty[i], 1);
-    }
-    for (int i = 0; i < PA_PIECES; ++i) {
-      mbar_init(&sh.bar_piece[i], 1);
-      mbar_init(&sh.bar_taken[i], 11);  // the warps that read it
-    }
-    mbar_init(&sh.bar_join, 4);
-    mbar_init(&sh.bar_joined, 4);
-    mbar_init(&sh.bar_end, 1);
-    mbar_init(&sh.bar_tail, 1);
-    mbar_init(&sh.bar_fix, 1);
-    fence_barrier_init();
+  if (tid < PagedShared<ST>::BARS)
+    mbar_init(&sh.bars[tid], tid < PagedShared<ST>::BARS_1 ? 1 : (tid < PagedShared<ST>::BARS_4 ? 4 : 11));
+  if (tid == 64) {
     prefetch_tensormap(&tmQ);
+    prefetch_tensormap(&tmQfew);
     prefetch_tensormap(&tmK);
     prefetch_tensormap(&tmV);
   }
+  fence_barrier_init();
   pdl_wait();
   if (warp == 9) {
     tmem_alloc(&sh.tmem, 512);
@@ -691,8 +708,6 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const int rows = piece.tokens * p.G;
         if (rows <= 16)
           ok = paged_few_piece<T, D, 16>(p, piece, sh, sQ, tS, tO, s, &sh.bar_q_empty[nq++ & 1], ns, no, nj, ng);
-        else if (rows <= 32)
-          ok = paged_few_piece<T, D, 32>(p, piece, sh, sQ, tS, tO, s, &sh.bar_q_empty[nq++ & 1], ns, no, nj, ng);
         else
           ok = paged_few_piece<T, D, 64>(p, piece, sh, sQ, tS, tO, s, &sh.bar_q_empty[nq++ & 1], ns, no, nj, ng);
         continue;
@@ -752,7 +767,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const int head = piece.h * p.G + rg;
         const size_t orow = static_cast<size_t>(token) * p.Hq + head;
         const size_t slot = static_cast<size_t>(whole ? 0 : piece.slot) * 256 + tile * 128 + r;
-#pragma unroll
+#pragma unroll 1
         for (int piece = 0; piece < D / 32; ++piece) {
           uint32_t oa[32];
           float v[32];
@@ -768,18 +783,16 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           }
           if (valid_row) {
             if (whole) {
-              uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + orow * D + piece * 32);
+              T* dst = static_cast<T*>(p.out) + orow * D + piece * 32;
+              uint32_t pk[16];
 #pragma unroll
-              for (int c = 0; c < 4; ++c)
-                dst[c] = make_uint4(pack_pair<T>(v[8 * c] * inv, v[8 * c + 1] * inv),
-                                    pack_pair<T>(v[8 * c + 2] * inv, v[8 * c + 3] * inv),
-                                    pack_pair<T>(v[8 * c + 4] * inv, v[8 * c + 5] * inv),
-                                    pack_pair<T>(v[8 * c + 6] * inv, v[8 * c + 7] * inv));
+              for (int j = 0; j < 16; ++j) pk[j] = pack_pair<T>(v[2 * j] * inv, v[2 * j + 1] * inv);
+              st_global_32b(dst, pk, p.out_32b);
+              st_global_32b(dst + 16, pk + 8, p.out_32b);
             } else {
-              float4* dst = reinterpret_cast<float4*>(p.ws_o + slot * D + piece * 32);
+              float* dst = p.ws_o + slot * D + piece * 32;
 #pragma unroll
-              for (int c = 0; c < 8; ++c)
-                dst[c] = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+              for (int c = 0; c < 4; ++c) st_global_32b(dst + 8 * c, reinterpret_cast<const uint32_t*>(v) + 8 * c, true);
             }
           }
         }
@@ -843,33 +856,36 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           }
           return id;
         };
-        auto load = [&](const CUtensorMap* map, int j, int id) {
+        // pair: K0 V0 K1 V1 ..; single (its streams start on two blocks): K0 K1 V0 K2 V1 .. V
+        int next_id = page_of(piece.j0), id = 0, id_before = 0, kk = 0, kv = 0;  // kk, kv: blocks of K, V so far
+#pragma unroll 1
+        for (int c = 0; ok && c < 2 * nblk; ++c) {
+          const bool is_k = kk < nblk && (pair ? kk == kv : kk < kv + 2);
+          const int j = piece.j0 + (is_k ? kk : kv);
+          if (is_k) {
+            id_before = id;
+            id = next_id;
+            next_id = page_of(j + 1);  // (on its way while this load waits for its stage)
+          }
+          const int mine = is_k || kk == kv + 1 ? id : id_before;
           const int st = nld % ST;
-          if (nld >= ST) ok = ok && __all_sync(0xffffffffu, mbar_wait(&sh.bar_empty[st], ((nld / ST) - 1) & 1));
-          if (!ok) return;
+          if (nld >= ST) ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_empty[st], ((nld / ST) - 1) & 1));
+          if (!ok) break;
           const int left = limit - j * PA_BN;
-          const int copies = left <= 0 ? 0 : min(per_block, (left + box - 1) / box);
+          const int copies = left <= 0 ? 0 : min(per_block, (left + box - 1) >> box_log2);
           if (lane == 0) mbar_arrive_expect_tx(&sh.bar_full[st], copies * copy_bytes);
           __syncwarp();
           if (lane < copies) {
             const int key = j * PA_BN + lane * box;
-            const int g = (id * p.Hkv + piece.h) * groups + ((key & ((1 << p.page_log2) - 1)) >> 3);
-            tma_load_4d(sKV + st * Tile::kv_bytes + lane * copy_bytes, map, &sh.bar_full[st], 0, 0, 0,
-                        id >= p.num_pages ? p.num_pages * p.Hkv * groups : g);
+            const int g = (mine * p.Hkv + piece.h) * groups + ((key & ((1 << p.page_log2) - 1)) >> 3);
+            tma_load_4d(sKV + st * Tile::kv_bytes + lane * copy_bytes, is_k ? &tmK : &tmV, &sh.bar_full[st], 0, 0, 0,
+                        mine >= p.num_pages ? p.num_pages * p.Hkv * groups : g);
           }
           ++nld;
-        };
-        int id0 = page_of(piece.j0), id1 = page_of(piece.j0 + 1);
-        if (ok) load(&tmK, piece.j0, id0);
-        for (int k = 0; ok && k < nblk; ++k) {
-          const int j = piece.j0 + k;
-          const int id2 = page_of(j + 2);
-          // a single reads K one block ahead (its two streams start on two blocks)
-          if (!pair && k + 1 < nblk) load(&tmK, j + 1, id1);
-          if (ok) load(&tmV, j, id0);
-          if (ok && pair && k + 1 < nblk) load(&tmK, j + 1, id1);
-          id0 = id1;
-          id1 = id2;
+          if (is_k)
+            ++kk;
+          else
+            ++kv;
         }
       }
       // never leave a copy in flight
@@ -1035,110 +1051,75 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       }
     } else if (warp == 10) {
       // ---------------- scheduler: the pieces of this CTA's share ----------------
-      // Costs of all requests first: chunks of 32, a request per lane, four
-      // chunks' lengths in flight at a time.
-      auto chunk_cost = [&](int n, int kv) -> long long {
-        const int items = (n + 2 * p.TQ - 1) / (2 * p.TQ);
-        int t0, nt, limit, nb, w;
-        long long cost = 0;
-        if (items == 1) {
-          paged_item(p, n, kv, 0, t0, nt, limit, nb, w);
-          cost = static_cast<long long>(nb) * w;
-        }
-        // a request of several items is summed by the whole warp
-        for (uint32_t many = __ballot_sync(0xffffffffu, items > 1); many != 0; many &= many - 1) {
-          const int src = __ffs(many) - 1;
-          const int n_ = __shfl_sync(0xffffffffu, n, src), kv_ = __shfl_sync(0xffffffffu, kv, src);
-          const int items_ = __shfl_sync(0xffffffffu, items, src);
-          long long sum = 0;
-          for (int i = lane; i < items_; i += 32) {
-            paged_item(p, n_, kv_, i, t0, nt, limit, nb, w);
-            sum += static_cast<long long>(nb) * w;
-          }
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          if (lane == src) cost = sum;
-        }
-        return cost * p.Hkv;
-      };
-      constexpr int AHEAD = 4;
-      auto lengths = [&](int b0, int* n, int* kv) {
-        int q0[AHEAD], q1[AHEAD];
-#pragma unroll
-        for (int c = 0; c < AHEAD; ++c) {
-          const int b = b0 + 32 * c + lane;
-          q0[c] = b < p.B ? __ldg(p.cu_q + b) : 0;
-          q1[c] = b < p.B ? __ldg(p.cu_q + b + 1) : 0;
-          kv[c] = b < p.B ? __ldg(p.kv_lens + b) : 0;
-        }
-#pragma unroll
-        for (int c = 0; c < AHEAD; ++c)
-          if (!paged_request(p, q0[c], q1[c], kv[c], n[c]) && cta == 0) std_set_error(STD_DEVERR_LENGTH);
-      };
-      long long total = 0;
-      long long cost[AHEAD];  // of the last four chunks seen: all of them when B <= 128
-      for (int b0 = 0; b0 < p.B; b0 += 32 * AHEAD) {
-        int n[AHEAD], kv[AHEAD];
-        lengths(b0, n, kv);
-#pragma unroll
-        for (int c = 0; c < AHEAD; ++c) {
-          cost[c] = b0 + 32 * c < p.B ? chunk_cost(n[c], kv[c]) : 0;
-          total += cost[c];
-        }
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-      // equal shares, of two blocks at least (a single's streams take one each)
-      const long long share = max((total + PA_CTAS - 1) / PA_CTAS, static_cast<long long>(2 * PA_W1));
-      const long long x0 = share * cta;
+      // Costs of the requests, 32 at a time, a request per lane (one of several
+      // items is summed by the whole warp): once for their total, and again for
+      // the place of this CTA's share.  (Rolled loops: on a first pass the
+      // instructions come from L2, and short code is what makes this quick.)
       PagedWalk walk;
       walk.rem = 0;
-      if (x0 < total) {
-        walk.rem = min(share, total - x0);
-        long long run = 0, off = 0;
-        walk.b = -1;
-        for (int b0 = 0; walk.b < 0 && b0 < p.B; b0 += 32 * AHEAD) {
-          int n[AHEAD], kv[AHEAD];
-          if (p.B > 32 * AHEAD) lengths(b0, n, kv);
-#pragma unroll
-          for (int c = 0; c < AHEAD; ++c) {
-            if (walk.b >= 0) continue;
-            const long long mine = p.B > 32 * AHEAD ? chunk_cost(n[c], kv[c]) : cost[c];
-            long long inc = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              const long long u = __shfl_up_sync(0xffffffffu, inc, o);
-              if (lane >= o) inc += u;
-            }
-            const uint32_t past = __ballot_sync(0xffffffffu, x0 < run + inc);
-            if (past != 0) {
-              const int src = __ffs(past) - 1;
-              walk.b = b0 + 32 * c + src;
-              off = x0 - __shfl_sync(0xffffffffu, run + inc - mine, src);
-            }
-            run += __shfl_sync(0xffffffffu, inc, 31);
+      int total = 0, share = 1, x0 = 0, off = 0;
+#pragma unroll 1
+      for (int pass = 0; pass < 2; ++pass) {
+        int run = 0;
+#pragma unroll 1
+        for (int b0 = 0; b0 < p.B; b0 += 32) {
+          const int b = b0 + lane;
+          int n = 0, kv = 0;
+          if (b < p.B) {
+            kv = __ldg(p.kv_lens + b);
+            if (!paged_request(p, __ldg(p.cu_q + b), __ldg(p.cu_q + b + 1), kv, n) && cta == 0)
+              std_set_error(STD_DEVERR_LENGTH);
           }
+          int cost = n > 0 && n <= 2 * p.TQ ? paged_item_cost(p, n, kv, 0) : 0;
+#pragma unroll 1
+          for (uint32_t many = __ballot_sync(0xffffffffu, n > 2 * p.TQ); many != 0; many &= many - 1) {
+            const int src = __ffs(many) - 1;
+            const int n_ = __shfl_sync(0xffffffffu, n, src), kv_ = __shfl_sync(0xffffffffu, kv, src);
+            int sum = 0;
+#pragma unroll 1
+            for (int i = lane; i * 2 * p.TQ < n_; i += 32) sum += paged_item_cost(p, n_, kv_, i);
+            sum = __reduce_add_sync(0xffffffffu, sum);
+            if (lane == src) cost = sum;
+          }
+          cost *= p.Hkv;
+          if (pass == 0) {
+            total += __reduce_add_sync(0xffffffffu, cost);
+            continue;
+          }
+          const int inc = warp_scan(cost, lane);
+          const uint32_t past = __ballot_sync(0xffffffffu, x0 < run + inc);
+          if (past != 0) {
+            const int src = __ffs(past) - 1;
+            walk.b = b0 + src;
+            off = x0 - __shfl_sync(0xffffffffu, run + inc - cost, src);
+            walk.rem = min(share, total - x0);
+            break;
+          }
+          run += __shfl_sync(0xffffffffu, inc, 31);
         }
-        if (walk.b < 0) walk.b = 0;  // (only if the lengths changed under the call)
+        if (pass == 0) {
+          // equal shares, of a two-block single at least (its streams take one block each)
+          share = max((total + PA_CTAS - 1) / PA_CTAS, ((2 + PA_OVER) * PA_W1) >> p.unit_log2);
+          if (total == 0 || cta >= (total + share - 1) / share) break;
+          x0 = share * cta;
+        }
+      }
+      if (walk.rem > 0) {
         walk.request(p);
-        int t0, nt, limit, nb, w;
-        long long head = 0;  // cost of one KV head of this request
-        if (walk.items == 1) {
-          paged_item(p, walk.n, walk.kv, 0, t0, nt, limit, nb, w);
-          head = static_cast<long long>(nb) * w;
-        } else {
-          for (int i = lane; i < walk.items; i += 32) {
-            paged_item(p, walk.n, walk.kv, i, t0, nt, limit, nb, w);
-            head += static_cast<long long>(nb) * w;
-          }
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) head += __shfl_xor_sync(0xffffffffu, head, o);
-        }
-        for (walk.h = 0; off >= head && walk.h + 1 < p.Hkv; ++walk.h) off -= head;
-        for (walk.i = 0; walk.i + 1 < walk.items; ++walk.i) {
-          paged_item(p, walk.n, walk.kv, walk.i, t0, nt, limit, nb, w);
-          const long long c = static_cast<long long>(nb) * w;
-          if (off < c) break;
+        // KV head and item: the items' costs, a run of `per` of them per lane
+        const int per = (walk.items + 31) / 32;
+        int sum = 0;
+#pragma unroll 1
+        for (int i = lane * per; i < min((lane + 1) * per, walk.items); ++i) sum += paged_item_cost(p, walk.n, walk.kv, i);
+        const int inc = warp_scan(sum, lane), head = __shfl_sync(0xffffffffu, inc, 31);
+        walk.h = off / head;
+        off -= walk.h * head;
+        const int src = __ffs(__ballot_sync(0xffffffffu, off < inc)) - 1;
+        off -= __shfl_sync(0xffffffffu, inc - sum, src);
+#pragma unroll 1
+        for (walk.i = src * per;; ++walk.i) {
+          const int c = paged_item_cost(p, walk.n, walk.kv, walk.i);
+          if (off < c || walk.i + 1 >= walk.items) break;
           off -= c;
         }
         walk.skip = off;
@@ -1161,10 +1142,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
         __syncwarp();
         if (more && walk.j0 == 0 && walk.j1 < walk.nb) {
-          // the share ends inside this item: block j lies with the CTA whose share
-          // holds cost j * w of the item
-          const long long start = x0 + share - walk.cut;
-          split.last_cta = static_cast<int>((start + static_cast<long long>(walk.nb - 1) * walk.w) / share);
+          // the share ends inside this item: a block lies with the CTA whose share holds its cost
+            const int start = x0 + share - walk.cut;
+          split.last_cta = (start + (((walk.nb - 1 + PA_OVER) * walk.w) >> p.unit_log2)) / share;
           split.token0 = walk.q0 + walk.t0;
           split.tokens = walk.nt;
           split.kvh = walk.h;
@@ -1183,8 +1163,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 }
 
 // Joins the pieces of the items that cuts divide: block x looks at the item
-// that CTA x's share ends inside.  A warp per row; out = sum_c w_c o_c / sum_c
-// w_c l_c with w_c = exp2(m_c - max m), pieces in CTA order.
+// that CTA x's share ends inside.  out = sum_c w_c o_c / sum_c w_c l_c with w_c =
+// exp2(m_c - max m), in a fixed order of the pieces.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnParams p) {
   pdl_launch_dependents();
@@ -1193,31 +1173,37 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnParams 
   const PagedSplit sp = p.splits[cta];
   if (sp.last_cta <= cta) return;
   const int n = sp.last_cta - cta + 1;
-  constexpr int PER = D / 32;    // columns per lane
+  constexpr int PER = D / 32;  // columns per lane
   constexpr int BATCH = 8;
-  for (int r = blockIdx.y * 8 + warp; r < 256; r += gridDim.y * 8) {
+  // Few pieces: a warp per row.  Many (long contexts split over many CTAs): the
+  // block's eight warps share a row's pieces, so that their loads are in flight
+  // together, and add up in warp order.
+  const bool shared = n > BATCH;
+  const int parts = shared ? 8 : 1, part = shared ? warp : 0;
+  __shared__ float s_acc[8][D], s_l[8], s_m[8];
+  const int r_first = shared ? blockIdx.y : blockIdx.y * 8 + warp, r_step = shared ? gridDim.y : gridDim.y * 8;
+  for (int r = r_first; r < 256; r += r_step) {
     const int rt = (r & 127) / p.G, t = (r >> 7) * p.TQ + rt;
     if (rt >= p.TQ || t >= sp.tokens) continue;
     // piece i is CTA cta + i's: its continued item (slot 0), or for the first the item begun there (slot 1)
     const size_t row0 = static_cast<size_t>(2 * cta) * 256 + r;
     auto at = [&](int i) { return row0 + static_cast<size_t>(2 * i + (i == 0 ? 1 : 0)) * 256; };
-    float m = -INFINITY;
-    for (int i = lane; i < n; i += 32) m = fmaxf(m, __ldcg(p.ws_ml + at(i)).x);
-    m = warp_max(m);
-    float l = 0.f, acc[PER];
+    float m = -INFINITY, l = 0.f, acc[PER];
 #pragma unroll
     for (int k = 0; k < PER; ++k) acc[k] = 0.f;
-    for (int i0 = 0; i0 < n; i0 += BATCH) {
+    for (int i0 = part; i0 < n; i0 += parts * BATCH) {
       float2 ml[BATCH];
       float o[BATCH][PER];
+      float mb = m;
 #pragma unroll
       for (int j = 0; j < BATCH; ++j) {
+        const int i = i0 + j * parts;
         ml[j] = make_float2(-INFINITY, 0.f);
 #pragma unroll
         for (int k = 0; k < PER; ++k) o[j][k] = 0.f;
-        if (i0 + j < n) {
-          ml[j] = __ldcg(p.ws_ml + at(i0 + j));
-          const float* src = p.ws_o + at(i0 + j) * D + lane * PER;
+        if (i < n) {
+          ml[j] = __ldcg(p.ws_ml + at(i));
+          const float* src = p.ws_o + at(i) * D + lane * PER;
           if constexpr (PER == 4) {
             const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
             o[j][0] = v.x, o[j][1] = v.y, o[j][2] = v.z, o[j][3] = v.w;
@@ -1228,6 +1214,13 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnParams 
         }
       }
 #pragma unroll
+      for (int j = 0; j < BATCH; ++j) mb = fmaxf(mb, ml[j].x);
+      const float scale = l != 0.f ? exp2f(m - mb) : 0.f;
+      l = l != 0.f ? l * scale : 0.f;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) acc[k] = l != 0.f ? acc[k] * scale : 0.f;
+      m = mb;
+#pragma unroll
       for (int j = 0; j < BATCH; ++j) {
         if (ml[j].y == 0.f) continue;  // a piece in which the row sees no key
         const float w = exp2f(ml[j].x - m);
@@ -1235,6 +1228,27 @@ __global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnParams 
 #pragma unroll
         for (int k = 0; k < PER; ++k) acc[k] += w * o[j][k];
       }
+    }
+    if (shared) {
+#pragma unroll
+      for (int k = 0; k < PER; ++k) s_acc[warp][lane * PER + k] = acc[k];
+      if (lane == 0) s_l[warp] = l, s_m[warp] = m;
+      __syncthreads();
+      if (warp == 0) {
+        for (int w = 0; w < 8; ++w) m = fmaxf(m, s_m[w]);
+        l = 0.f;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) acc[k] = 0.f;
+        for (int w = 0; w < 8; ++w) {
+          if (s_l[w] == 0.f) continue;
+          const float f = exp2f(s_m[w] - m);
+          l += f * s_l[w];
+#pragma unroll
+          for (int k = 0; k < PER; ++k) acc[k] += f * s_acc[w][lane * PER + k];
+        }
+      }
+      __syncthreads();  // before the next row's values
+      if (warp != 0) continue;
     }
     const float inv = l != 0.f ? 1.f / l : 0.f;
     const size_t orow = static_cast<size_t>(sp.token0 + t) * p.Hq + sp.kvh * p.G + (r & 127) % p.G;
@@ -1287,7 +1301,7 @@ static int paged_attn_launch(const CUtensorMap& tq, const CUtensorMap& tqf, cons
     return 4;
   // rows that an item can have: all of a pair's 256, or those of all the tokens there are
   const int rows = p.T > p.TQ ? 256 : p.T * p.G;
-  const dim3 mgrid(stdb::PA_CTAS, rows >= 64 ? 8 : (rows + 7) / 8);
+  const dim3 mgrid(stdb::PA_CTAS, rows < 8 ? rows : 8);
   if (launch_pdl(stdb::paged_merge_kernel<T, D>, mgrid, dim3(256), 0, s, p) != cudaSuccess) return 4;
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
@@ -1310,7 +1324,7 @@ extern "C" int std_paged_attn(const void* q, const void* k_pages, const void* v_
       kv_lens == nullptr || out == nullptr || q == out)
     return 1;
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out)) return 1;
-  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < std_paged_attn_workspace_bytes(D)) return 5;
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 31) != 0 || workspace_bytes < std_paged_attn_workspace_bytes(D)) return 5;
   const int G = Hq / Hkv, TQ = 128 / G, TQ_few = stdb::PA_FEW / G;
   CUtensorMap tq, tqf, tk, tv;
   {
@@ -1348,10 +1362,16 @@ extern "C" int std_paged_attn(const void* q, const void* k_pages, const void* v_
   p.Hkv = Hkv;
   p.G = G;
   p.TQ = TQ;
+  // total cost of the calls that these shapes allow, and its unit
+  const double most = (static_cast<double>(T) / (2 * TQ) + B) * Hkv *
+                      (static_cast<double>(max_blocks) * page_size / stdb::PA_BN + stdb::PA_OVER + 1) * stdb::PA_W2;
+  p.unit_log2 = 0;
+  while (most / (1ll << p.unit_log2) + (static_cast<double>(T) / (2 * TQ) + B) * Hkv > 1.0e9) ++p.unit_log2;
   p.TQ_few = TQ_few;
   p.causal = causal != 0 ? 1 : 0;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.out = out;
+  p.out_32b = (reinterpret_cast<uintptr_t>(out) & 31) == 0;
   p.lse = lse;
   char* ws = static_cast<char*>(workspace);
   p.ws_o = reinterpret_cast<float*>(ws);
