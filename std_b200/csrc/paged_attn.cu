@@ -9,8 +9,9 @@
 // whole tokens per 128-row tile.  An item is one KV head's span of up to 2 TQ
 // tokens of one request: a pair of tiles that share every K/V block or, when at
 // most TQ tokens are left, a single one.  Keys come in blocks of 128.
-//   S = Q K^T     tcgen05.mma M=128 N=128, Q and K from shared memory
-//   P = exp2(S * scale * log2e - m), 16 bits, written over S in TMEM
+//   S = Q K^T     tcgen05.mma M=128, two halves of N=64 keys, Q and K from
+//                 shared memory
+//   P = exp2(S * scale * log2e - m), 16 bits, each half written over its S in TMEM
 //   O += P V      tcgen05.mma with P as the A operand in TMEM, V MN-major
 // Two softmax warpgroups each own a stream of steps with an S and an O of its
 // own in TMEM: in a pair, stream s is tile s; in a single, stream s takes the
@@ -49,7 +50,7 @@
 namespace stdb {
 
 constexpr int PA_CTAS = 148;     // one CTA per SM
-constexpr int PA_THREADS = 384;  // 2 softmax warpgroups; TMA, MMA, scheduler and clearing warp
+constexpr int PA_THREADS = 384;  // 2 softmax warpgroups; TMA, two MMA and a scheduler warp
 // Registers after the split: 2 * 128 * 208 + 128 * 88 = 384 * 168, the launch's total.
 constexpr int PA_REGS_SOFTMAX = 208, PA_REGS_OTHER = 88;
 constexpr int PA_BN = 128;       // keys per block
@@ -211,16 +212,21 @@ STD_DEV void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, 
 template <int ST>
 struct PagedShared {
   // mbarriers, by the arrivals that complete a phase
-  static constexpr int BARS_1 = 11 + 2 * ST + PA_PIECES, BARS_4 = BARS_1 + 8, BARS = BARS_4 + PA_PIECES;
+  static constexpr int BARS_1 = 12 + ST + PA_PIECES, BARS_2 = BARS_1 + ST, BARS_3 = BARS_2 + 2,
+                       BARS_4 = BARS_3 + 8, BARS = BARS_4 + PA_PIECES;
   union {
     uint64_t bars[BARS];
     struct {
       // one
-      uint64_t bar_q_full[2], bar_q_empty[2];  // query slots
-      uint64_t bar_s[2], bar_o[2];             // per stream: S there, O complete
-      uint64_t bar_tail, bar_fix, bar_end;     // a tail's V there, its rows cleared; all MMAs done
-      uint64_t bar_full[ST], bar_empty[ST];    // K/V ring
+      uint64_t bar_q_full[2];                  // query slots
+      uint64_t bar_s[2][2], bar_o[2];          // per stream: S's halves there, O complete
+      uint64_t bar_tail[2], bar_end[2];        // a tail's V there; all MMAs done
+      uint64_t bar_full[ST];                   // K/V ring
       uint64_t bar_piece[PA_PIECES];
+      // two: both MMA threads have seen the load, and its readers are done
+      uint64_t bar_empty[ST];
+      // three: both MMA threads have seen the tile, and its reader is done
+      uint64_t bar_q_empty[2];
       // four (a stream's warps)
       uint64_t bar_p[2], bar_p2[2];   // P's halves there
       uint64_t bar_join, bar_joined;  // a single's two streams
@@ -365,32 +371,47 @@ STD_DEV float2 ex2_fma2(uint64_t y2) {
   return out;
 }
 
-// One step of a whole tile's softmax: S (128 columns of this thread's row) to
-// P, with the row's running m and l.  Raises sh's barriers for P's halves.
+// Clears the V rows of a tail that no query sees, up to the multiple of 16 at
+// which the products stop (rows last .. of the stage sV), by a stream's 128 threads.
+template <int D>
+STD_DEV void paged_clear_tail(uint8_t* sV, int last, int thread) {
+  constexpr int HALVES = D / 64;
+  for (int i = thread; i < (16 - (last & 15)) * HALVES * 8; i += 128) {
+    const int r = last + i / (HALVES * 8), ch = i % (HALVES * 8);
+    *reinterpret_cast<uint4*>(sV + (r >> 3) * (HALVES * 1024) + (ch >> 3) * 1024 + (r & 7) * 128 + (ch & 7) * 16) =
+        make_uint4(0, 0, 0, 0);
+  }
+  fence_async_smem();
+}
+
+// Half a step of a whole tile's softmax: 64 columns of S to P, with the row's
+// running m and l.  bar_next: the barrier (phase parity `next`) after which the
+// stream's products issued so far are complete.  False when a wait ran out.
 template <typename T, int D>
-STD_DEV void paged_softmax_step(uint32_t tS, uint32_t tO, float sc, int nvis, float& m_run, float& l_run,
-                                uint64_t* bar_p, uint64_t* bar_p2, int lane) {
-  uint32_t x[PA_BN];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, x + c * 32);
+STD_DEV bool paged_softmax_half(uint32_t tS, uint32_t tO, float sc, int nvis, float& m_run, float& l_run,
+                                uint64_t* bar_next, uint32_t next) {
+  constexpr int N = PA_BN / 2;
+  uint32_t x[N];
+  tmem_ld32(tS, x);
+  tmem_ld32(tS + 32, x + 32);
   tmem_wait_ld();
-  if (__any_sync(0xffffffffu, nvis < PA_BN)) {
+  if (__any_sync(0xffffffffu, nvis < N)) {
 #pragma unroll
-    for (int j = 0; j < PA_BN; ++j)
+    for (int j = 0; j < N; ++j)
       if (j >= nvis) x[j] = 0xff800000u;  // -inf
   }
   float m4[4];
 #pragma unroll
   for (int c = 0; c < 4; ++c) m4[c] = fmaxf(__uint_as_float(x[c]), __uint_as_float(x[4 + c]));
 #pragma unroll
-  for (int j = 8; j < PA_BN; j += 8)
+  for (int j = 8; j < N; j += 8)
 #pragma unroll
     for (int c = 0; c < 4; ++c) m4[c] = max3(m4[c], __uint_as_float(x[j + c]), __uint_as_float(x[j + 4 + c]));
   const float m_c = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;  // scale > 0
-  // This block's S is issued after the stream's previous P V, and its barrier
-  // covers all MMAs before it: O is at rest here.
   const bool need = m_run != -INFINITY && m_c > m_run + PA_RESCALE;
   if (__any_sync(0xffffffffu, need)) {
+    if (!__all_sync(0xffffffffu, mbar_wait(bar_next, next & 1))) return false;  // O at rest
+    tc_fence_after();
     const float alpha = need ? exp2f(m_run - m_c) : 1.0f;
     uint32_t o[32];
 #pragma unroll 1
@@ -411,33 +432,27 @@ STD_DEV void paged_softmax_step(uint32_t tS, uint32_t tO, float sc, int nvis, fl
   const float nm = m_run == -INFINITY ? 0.f : -m_run;
   const uint64_t sc2 = f2_make(sc, sc), nm2 = f2_make(nm, nm);
   uint64_t l2[2] = {f2_make(l_run, 0.f), f2_make(0.f, 0.f)};
+  uint32_t pk[N / 2];
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint32_t pk[16];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const uint64_t y = f2_fma(f2_make(__uint_as_float(x[c * 32 + 2 * j]), __uint_as_float(x[c * 32 + 2 * j + 1])), sc2, nm2);
-      float2 e;
-      if (PA_POLY > 0 && j % PA_POLY == PA_POLY - 1) {
-        e = ex2_fma2(y);
-      } else {
-        e = f2_split(y);
-        e.x = ex2_approx(e.x);
-        e.y = ex2_approx(e.y);
-      }
-      l2[j & 1] = f2_add(l2[j & 1], f2_make(e.x, e.y));
-      pk[j] = pack_pair<T>(e.x, e.y);
+  for (int j = 0; j < N / 2; ++j) {
+    const uint64_t y = f2_fma(f2_make(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), sc2, nm2);
+    float2 e;
+    if (PA_POLY > 0 && j % PA_POLY == PA_POLY - 1) {
+      e = ex2_fma2(y);
+    } else {
+      e = f2_split(y);
+      e.x = ex2_approx(e.x);
+      e.y = ex2_approx(e.y);
     }
-    tmem_st16(tS + c * 16, pk);
-    if (c & 1) {
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(c == 1 ? bar_p : bar_p2);
-    }
+    l2[j & 1] = f2_add(l2[j & 1], f2_make(e.x, e.y));
+    pk[j] = pack_pair<T>(e.x, e.y);
   }
+  tmem_st32(tS, pk);
+  tmem_wait_st();
+  tc_fence_before();
   const float2 l = f2_split(f2_add(l2[0], l2[1]));
   l_run = l.x + l.y;
+  return true;
 }
 
 // Combines N values of each lane over the warp: halving the rows a lane keeps at
@@ -465,14 +480,15 @@ STD_DEV int warp_reduce_rows(float* v, int lane, Op op) {
 // A piece with few rows, for one warp of stream s (thread = key of the block,
 // N >= the piece's rows columns).  ns, no, nj, ng: phases used so far of the
 // stream's S, O, join and group barriers; bar_q_empty: its query slot's.  False
-// when a wait ran out.
+// when a wait ran out.  sV: the stage of the piece's last V; ntail: tails cleared.
 //
 // m (sh.ref) is set to the row's maximum over the first block and raised when a
 // score passes it by 2^8, on all four warps: they vote at every block.  The keys
 // a row sees are a prefix, so a row without one in the first block has none.
 template <typename T, int D, int N, int ST>
 STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, PagedShared<ST>& sh, uint8_t* sQ,
-                             uint32_t tS, uint32_t tO, int s, uint64_t* bar_q_empty, uint32_t& ns, uint32_t& no, uint32_t& nj,
+                             uint8_t* sV, uint32_t tS, uint32_t tO, int s, uint64_t* bar_q_empty, uint32_t& ntail,
+                             uint32_t& ns, uint32_t& no, uint32_t& nj,
                              uint32_t& ng) {
   const int tid = threadIdx.x, lane = tid & 31, w = (tid >> 5) & 3, key = tid & 127;
   const int rows = piece.tokens * p.G, steps = (piece.nblk - s + 1) >> 1;
@@ -492,7 +508,7 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
   for (int n = 0; n < N; ++n) l[n] = 0.f;
 #pragma unroll 1
   for (int k = 0; k < steps; ++k, ++ns) {
-    if (!__all_sync(0xffffffffu, mbar_wait(&sh.bar_s[s], ns & 1))) return false;
+    if (!__all_sync(0xffffffffu, mbar_wait(&sh.bar_s[s][0], ns & 1))) return false;
     tc_fence_after();
     float y[N];
     tmem_ld_cols<N>(tS, reinterpret_cast<uint32_t*>(y));
@@ -561,6 +577,11 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
       *reinterpret_cast<uint4*>(row_p + (((n >> 3) ^ (key & 7)) << 4)) =
           make_uint4(pack_pair<T>(e[0], e[1]), pack_pair<T>(e[2], e[3]), pack_pair<T>(e[4], e[5]),
                      pack_pair<T>(e[6], e[7]));
+    }
+    const int left = piece.limit - (pos - key);
+    if (left < PA_BN && (left & 15) != 0) {  // the last block, which ends inside a 16-key step
+      if (!__all_sync(0xffffffffu, mbar_wait(&sh.bar_tail[s], ntail++ & 1))) return false;
+      paged_clear_tail<D>(sV, left, key);
     }
     fence_async_smem();
     tc_fence_before();
@@ -658,7 +679,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   __shared__ PagedShared<ST> sh;
 
   if (tid < PagedShared<ST>::BARS)
-    mbar_init(&sh.bars[tid], tid < PagedShared<ST>::BARS_1 ? 1 : (tid < PagedShared<ST>::BARS_4 ? 4 : 11));
+    mbar_init(&sh.bars[tid], tid < PagedShared<ST>::BARS_1   ? 1
+                             : tid < PagedShared<ST>::BARS_2 ? 2
+                             : tid < PagedShared<ST>::BARS_3 ? 3
+                             : tid < PagedShared<ST>::BARS_4 ? 4
+                                                             : 11);
   if (tid == 64) {
     prefetch_tensormap(&tmQ);
     prefetch_tensormap(&tmQfew);
@@ -698,18 +723,22 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const uint32_t tS = trow + s * 128, tO = trow + T_O + s * 128;
     const int rt = r / p.G, rg = r % p.G;  // token and head of this row in its tile
     const float sc = p.scale_log2;
-    uint32_t npiece = 0, ns = 0, no = 0, nj = 0, ng = 0, nq = 0;  // pieces, steps, results, joins, group syncs, query tiles so far
+    uint32_t npiece = 0, ns = 0, no = 0, nj = 0, ng = 0;  // pieces, steps, results, joins, group syncs so far
+    uint32_t ns1 = 0;                              // steps' second halves
+    uint32_t nq = 0, ntail = 0, nld = 0;           // query tiles, tails cleared, loads so far
     bool ok = true;
     PagedPiece piece;
     while (ok && next_piece(npiece, piece)) {
       const int nblk = piece.nblk;
       const bool pair = piece.tokens > p.TQ;
+      nld += 2 * nblk;
+      uint8_t* sV = sKV + (nld - 1) % ST * Tile::kv_bytes;  // the stage of the piece's last V
       if (piece.tokens <= p.TQ_few) {
         const int rows = piece.tokens * p.G;
         if (rows <= 16)
-          ok = paged_few_piece<T, D, 16>(p, piece, sh, sQ, tS, tO, s, &sh.bar_q_empty[nq++ & 1], ns, no, nj, ng);
+          ok = paged_few_piece<T, D, 16>(p, piece, sh, sQ, sV, tS, tO, s, &sh.bar_q_empty[nq++ & 1], ntail, ns, no, nj, ng);
         else
-          ok = paged_few_piece<T, D, 64>(p, piece, sh, sQ, tS, tO, s, &sh.bar_q_empty[nq++ & 1], ns, no, nj, ng);
+          ok = paged_few_piece<T, D, 64>(p, piece, sh, sQ, sV, tS, tO, s, &sh.bar_q_empty[nq++ & 1], ntail, ns, no, nj, ng);
         continue;
       }
       nq += pair ? 2 : 1;
@@ -721,18 +750,37 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       const int limit = p.causal ? min(piece.limit, piece.first + t) : piece.limit;
       const int steps = pair ? nblk : (nblk - s + 1) >> 1;
       float m_run = -INFINITY, l_run = 0.f;
-      for (int k = 0; k < steps; ++k, ++ns) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_s[s], ns & 1));
+#pragma unroll 1
+      for (int h = 0; ok && h < 2 * steps; ++h) {  // half steps
+        const int half = h & 1, k = h >> 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_s[s][half], (half == 0 ? ns : ns1) & 1));
         if (!ok) break;
+        const int k0 = (piece.j0 + (pair ? k : 2 * k + s)) * PA_BN, left = piece.limit - k0;
+        if (half == 0) {
+          ++ns;
+          if (left < PA_BN && (left & 15) != 0) {
+            // the last block, which ends inside a 16-key step (both streams of a pair
+            // clear its rows, each before its own product)
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_tail[s], ntail++ & 1));
+            if (!ok) break;
+            paged_clear_tail<D>(sV, left, r);
+            __syncwarp();
+          }
+        } else {
+          ++ns1;
+        }
         if (live) {
           tc_fence_after();
-          const int nvis = limit - (piece.j0 + (pair ? k : 2 * k + s)) * PA_BN;  // visible keys of this block
-          paged_softmax_step<T, D>(tS, tO, sc, nvis, m_run, l_run, &sh.bar_p[s], &sh.bar_p2[s], lane);
-        } else if (lane == 0) {
-          mbar_arrive(&sh.bar_p[s]);
-          mbar_arrive(&sh.bar_p2[s]);
+          // (limit - k0: visible keys of this block.)  The products so far are complete
+          // once the other half's next S is: it was issued after the last of them.
+          ok = paged_softmax_half<T, D>(tS + half * (PA_BN / 2), tO, sc, limit - k0 - half * (PA_BN / 2), m_run, l_run,
+                                        &sh.bar_s[s][half ^ 1], half == 0 ? ns1 : ns);
+          if (!ok) break;
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(half == 0 ? &sh.bar_p[s] : &sh.bar_p2[s]);
       }
+      if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_s[s][0], ns++ & 1));  // (the commit after the last P V)
       // ---- the item's result ----
       if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_o[s], no++ & 1));
       if (!ok) break;
@@ -811,6 +859,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           if (lane == 0) mbar_arrive(&sh.bar_joined);
         } else {
           ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_joined, nj & 1));
+          // both streams are done, and with them the query slot
+          if (ok && tid == 128) mbar_arrive(&sh.bar_q_empty[(nq - 1) & 1]);
         }
         ++nj;
       }
@@ -891,165 +941,200 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       // never leave a copy in flight
       for (uint32_t c = nld < ST ? 0 : nld - ST; c < nld; ++c) mbar_wait(&sh.bar_full[c % ST], (c / ST) & 1);
       for (uint32_t c = nq < 2 ? 0 : nq - 2; c < nq; ++c) mbar_wait(&sh.bar_q_full[c & 1], (c >> 1) & 1);
-    } else if (warp == 9) {
-      // ---------------- MMA issuer: one thread ----------------
+    } else if (warp < 11) {
+      // ---------------- MMA issuers: one thread per stream ----------------
+      // A stream's S and P V go out in order from one thread, which is what lets S
+      // be written over the P that its last P V read.  Per stream, since issuing a
+      // step (waits, commits, 16 MMAs beside busy softmax warps) takes one thread
+      // about as long as the tensor core needs for two.
+      const int s = warp - 9;
       if (elect_one()) {
-        constexpr uint32_t idS = paged_idesc<T>(128, PA_BN, 0, 0);
+        constexpr uint32_t idS = paged_idesc<T>(128, PA_BN / 2, 0, 0);
         constexpr uint32_t idO = paged_idesc<T>(128, D, 0, 1);
         // (a descriptor's low bits are the address / 16, so offsets are added to it)
-        const uint64_t dKV = sdesc_sw128(smem_u32(sKV), 16, HALVES * 1024);   // K-major
+        const uint64_t dKV = sdesc_sw128(smem_u32(sKV), 16, HALVES * 1024);    // K-major
         const uint64_t dVm = sdesc_sw128(smem_u32(sKV), 1024, HALVES * 1024);  // MN-major
         // V as the A operand: D 64 has no second block of 64 columns, rows 64..127 repeat the first
         const uint64_t dVa = sdesc_sw128(smem_u32(sKV), HALVES == 2 ? 1024 : 0, HALVES * 1024);
-        const uint64_t dQ0 = sdesc_sw128(smem_u32(sQ), 16, 1024), dP0 = sdesc_sw128(smem_u32(sQ + PA_PT), 16, 1024);
-        uint32_t npiece = 0, nfix = 0, nq = 0;  // pieces, blocks with cleared V rows, query tiles so far
-        uint32_t st0 = 0, ph0 = 0;              // ring position of the piece's first load
-        uint32_t np[2] = {0, 0}, np2[2] = {0, 0};
-        auto advance = [](uint32_t& st, uint32_t& ph, int by) {
-          st += by;
-          if (st >= ST) {
-            st -= ST;
-            ph ^= 1;
-          }
-        };
-        PagedPiece piece;
-        bool ok = true;
+        const uint64_t dQ0 = sdesc_sw128(smem_u32(sQ), 16, 1024);
+        const uint64_t dP = sdesc_sw128(smem_u32(sQ + s * PA_SLOT + PA_PT), 16, 1024);
+        const uint32_t tS = tmem + s * 128, tO = tmem + T_O + s * 128;
+        uint32_t npiece = 0, nq = 0;      // pieces, query tiles so far
+        uint32_t st = 0, ph = 0;                // ring position of the next load, its turn's parity
+        uint32_t np = 0, np2 = 0;               // P halves so far
         for (;;) {
           const int ip = npiece % PA_PIECES;
           if (!mbar_wait(&sh.bar_piece[ip], (npiece / PA_PIECES) & 1)) break;
-          piece = sh.piece[ip];
+          const PagedPiece piece = sh.piece[ip];
           mbar_arrive(&sh.bar_taken[ip]);
           ++npiece;
           const int nblk = piece.nblk;
           if (nblk <= 0) break;
           const bool pair = piece.tokens > p.TQ, few = piece.tokens <= p.TQ_few;
-          const int steps = pair ? 2 * nblk : nblk;
-          const int n_few = paged_few_cols(piece.tokens * p.G);
-          const uint32_t idSt = paged_idesc<T>(128, n_few, 0, 0), idOt = paged_idesc<T>(128, n_few, 1, 1);
           // visible keys of the last block: products stop at the next multiple of 16
           const int last = min(PA_BN, piece.limit - (piece.j0 + nblk - 1) * PA_BN);
-          uint32_t kst = st0, kph = ph0, vst = st0, vph = ph0;
-          advance(vst, vph, pair || nblk == 1 ? 1 : 2);
-          // S runs two steps ahead: S0 S1 PV0 S2 PV1 S3 ...
-#pragma unroll 1
-          for (int v = 0; ok && v < steps + 2; ++v) {
-            const int s = v & 1;
-            const uint32_t tS = tmem + s * 128, tO = tmem + T_O + s * 128;
-            if (v >= 2) {
-              const int u = v - 2, k = pair ? u >> 1 : u;
-              const bool tail = k + 1 == nblk && last < PA_BN;
-              const int ksteps = tail ? (last + 15) >> 4 : PA_BN / 16;
-              const uint32_t off = vst * (Tile::kv_bytes / 16);
-              if (!pair || s == 0) {
-                ok = mbar_wait(&sh.bar_full[vst], vph);
-                if (ok && tail && (last & 15) != 0) {
-                  mbar_arrive(&sh.bar_tail);
-                  ok = mbar_wait(&sh.bar_fix, nfix++ & 1);
-                }
+          const int last_steps = (last + 15) >> 4;
+          // query tiles: a pair's stream has its own, a single's share one (whose
+          // third release comes from the softmax)
+          const uint32_t qs = (nq + (pair ? s : 0)) & 1;
+          bool ok = mbar_wait(&sh.bar_q_full[nq & 1], (nq >> 1) & 1);
+          ++nq;
+          if (pair) {
+            ok = ok && mbar_wait(&sh.bar_q_full[nq & 1], (nq >> 1) & 1);
+            ++nq;
+          }
+          mbar_arrive(&sh.bar_q_empty[pair ? qs ^ 1 : qs]);
+          const uint64_t dQ = dQ0 + qs * (PA_SLOT / 16);
+          // Load `index` of the piece, in its stage `at`.  Loads are waited for in ring
+          // order whoever uses them, and not given back before both threads have
+          // passed them: a barrier's parity tells neighbouring phases apart, no more,
+          // so neither thread may fall a turn behind.
+          int pos = 0;
+          uint32_t at = 0;
+          auto take = [&](int index) -> bool {
+            for (;; ++pos) {
+              if (!mbar_wait(&sh.bar_full[st], ph)) return false;
+              at = st;
+              if (++st == ST) {
+                st = 0;
+                ph ^= 1;
               }
-              ok = ok && mbar_wait(&sh.bar_p[s], np[s]++ & 1);
-              if (!ok) break;
-              tc_fence_after();
-              if (few) {
-                const uint64_t dP = dP0 + s * (PA_SLOT / 16);
-                umma_bf16(tO, dVa + off, dP, idOt, u >= 2 ? 1u : 0u);
-                if (!tail) {
-#pragma unroll
-                  for (int ks = 1; ks < PA_BN / 16; ++ks)
-                    umma_bf16(tO, dVa + off + ks * (HALVES * 2048 / 16), dP + ks * (2048 / 16), idOt, 1u);
-                } else {
-#pragma unroll 1
-                  for (int ks = 1; ks < ksteps; ++ks)
-                    umma_bf16(tO, dVa + off + ks * (HALVES * 2048 / 16), dP + ks * (2048 / 16), idOt, 1u);
-                }
-              } else {
-                // the first half of P, then (its own barrier) the second
-                umma_bf16_ts(tO, tS, dVm + off, idO, u >= 2 ? 1u : 0u);
-                if (!tail) {
-#pragma unroll
-                  for (int ks = 1; ks < PA_BN / 32; ++ks)
-                    umma_bf16_ts(tO, tS + ks * 8, dVm + off + ks * (HALVES * 2048 / 16), idO, 1u);
-                } else {
-#pragma unroll 1
-                  for (int ks = 1; ks < min(ksteps, PA_BN / 32); ++ks)
-                    umma_bf16_ts(tO, tS + ks * 8, dVm + off + ks * (HALVES * 2048 / 16), idO, 1u);
-                }
-                ok = mbar_wait(&sh.bar_p2[s], np2[s]++ & 1);
-                if (!ok) break;
-                tc_fence_after();
-                if (!tail) {
-#pragma unroll
-                  for (int ks = PA_BN / 32; ks < PA_BN / 16; ++ks)
-                    umma_bf16_ts(tO, tS + ks * 8, dVm + off + ks * (HALVES * 2048 / 16), idO, 1u);
-                } else {
-#pragma unroll 1
-                  for (int ks = PA_BN / 32; ks < ksteps; ++ks)
-                    umma_bf16_ts(tO, tS + ks * 8, dVm + off + ks * (HALVES * 2048 / 16), idO, 1u);
-                }
-              }
-              if (!pair || s == 1) {
-                umma_commit(&sh.bar_empty[vst]);
-                advance(vst, vph, pair || k + 2 < nblk ? 2 : 1);
-              }
-              if (u + 2 >= steps) umma_commit(&sh.bar_o[s]);
+              if (pos == index) break;
+              mbar_arrive(&sh.bar_empty[at]);
             }
-            if (v < steps) {
-              const uint32_t qi = nq + (pair ? s : 0), qs = qi & 1;
-              if (!pair || s == 0) ok = mbar_wait(&sh.bar_full[kst], kph);
-              if (v == 0 || (pair && v == 1)) ok = ok && mbar_wait(&sh.bar_q_full[qs], (qi >> 1) & 1);
-              if (!ok) break;
-              tc_fence_after();
-              const uint64_t dK = dKV + kst * (Tile::kv_bytes / 16), dQ = dQ0 + qs * (PA_SLOT / 16);
-              if (few) {
+            ++pos;
+            return true;
+          };
+          // pair: K0 V0 K1 V1 ..; single: K0 K1 V0 K2 V1 .. V, stream s using blocks s, s + 2 ..
+          const int step = pair ? 1 : 2;
+          int k = pair ? 0 : s;
+          if (ok && k < nblk) {
+            ok = take(pair || k == 0 ? 0 : 1);
+            if (few) {
+              const uint32_t n_few = paged_few_cols(piece.tokens * p.G);
+              const uint32_t idSt = paged_idesc<T>(128, n_few, 0, 0), idOt = paged_idesc<T>(128, n_few, 1, 1);
+#pragma unroll 1
+              for (; ok; k += 2) {
+                tc_fence_after();
+                const uint64_t dK = dKV + at * (Tile::kv_bytes / 16);
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks)
                   umma_bf16(tS, dK + ((ks >> 2) * 1024 + (ks & 3) * 32) / 16,
                             dQ + ((ks >> 2) * 8192 + (ks & 3) * 32) / 16, idSt, ks > 0 ? 1u : 0u);
-              } else {
+                umma_commit(&sh.bar_s[s][0]);
+                umma_commit(&sh.bar_empty[at]);
+                const bool end = k + 1 == nblk;
+                ok = take(end ? 2 * nblk - 1 : 2 * k + 2);
+                if (!ok) break;
+                if (end && (last & 15) != 0) mbar_arrive(&sh.bar_tail[s]);
+                ok = mbar_wait(&sh.bar_p[s], np++ & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t dV = dVa + at * (Tile::kv_bytes / 16);
+                const int ksteps = end ? last_steps : PA_BN / 16;
+                uint32_t more = k > 1 ? 1u : 0u;
+#pragma unroll 2
+                for (int ks = 0; ks < ksteps; ++ks, more = 1u)
+                  umma_bf16(tO, dV + ks * (HALVES * 2048 / 16), dP + ks * (2048 / 16), idOt, more);
+                umma_commit(&sh.bar_empty[at]);
+                if (k + 2 >= nblk) break;
+                ok = take(2 * k + 3);
+              }
+              if (ok) umma_commit(&sh.bar_o[s]);
+            } else {
+              // S in halves of 64 keys, each a block ahead of its half's product:
+              // Sa0 Sb0, PVa0 Sa1 PVb0 Sb1, PVa1 Sa2 ...  The softmax always has a half
+              // ready while the other is in the tensor core.
+              auto s_half = [&](uint32_t stage, int half) {
+                const uint64_t dK = dKV + stage * (Tile::kv_bytes / 16) + half * (8 * HALVES * 1024 / 16);
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks)
-                  umma_bf16(tS, dQ + ((ks >> 2) * 16384 + (ks & 3) * 32) / 16,
+                  umma_bf16(tS + half * 64, dQ + ((ks >> 2) * 16384 + (ks & 3) * 32) / 16,
                             dK + ((ks >> 2) * 1024 + (ks & 3) * 32) / 16, idS, ks > 0 ? 1u : 0u);
+                umma_commit(&sh.bar_s[s][half]);
+              };
+              if (ok) {
+                tc_fence_after();
+                s_half(at, 0);
+                s_half(at, 1);
+                umma_commit(&sh.bar_empty[at]);
+                if (k + step >= nblk && pair) {
+                  umma_commit(&sh.bar_q_empty[qs]);
+                  umma_commit(&sh.bar_q_empty[qs]);
+                }
               }
-              umma_commit(&sh.bar_s[s]);
-              if (!pair || s == 1) {
-                umma_commit(&sh.bar_empty[kst]);
-                advance(kst, kph, pair || v > 0 ? 2 : 1);
+              uint32_t more = 0;
+#pragma unroll 1
+              for (; ok; k += step) {
+                const bool end = k + 1 == nblk, has_next = k + step < nblk;
+                ok = take(pair ? 2 * k + 1 : (end ? 2 * nblk - 1 : 2 * k + 2));
+                if (!ok) break;
+                const uint32_t at_v = at;
+                const uint64_t dV = dVm + at_v * (Tile::kv_bytes / 16);
+                if (end && (last & 15) != 0) mbar_arrive(&sh.bar_tail[s]);
+                ok = mbar_wait(&sh.bar_p[s], np++ & 1);
+                if (!ok) break;
+                tc_fence_after();
+                if (!end) {
+                  umma_bf16_ts(tO, tS, dV, idO, more);
+#pragma unroll
+                  for (int ks = 1; ks < PA_BN / 32; ++ks)
+                    umma_bf16_ts(tO, tS + ks * 8, dV + ks * (HALVES * 2048 / 16), idO, 1u);
+                } else {
+#pragma unroll 1
+                  for (int ks = 0; ks < min(last_steps, PA_BN / 32); ++ks)
+                    umma_bf16_ts(tO, tS + ks * 8, dV + ks * (HALVES * 2048 / 16), idO, more | (ks > 0 ? 1u : 0u));
+                }
+                more = 1u;
+                if (has_next) {
+                  ok = take(pair ? 2 * k + 2 : 2 * k + 3);
+                  if (!ok) break;
+                  tc_fence_after();
+                  s_half(at, 0);
+                } else {
+                  umma_commit(&sh.bar_s[s][0]);  // for a second half that rescales O
+                }
+                ok = mbar_wait(&sh.bar_p2[s], np2++ & 1);
+                if (!ok) break;
+                tc_fence_after();
+                if (!end) {
+#pragma unroll
+                  for (int ks = PA_BN / 32; ks < PA_BN / 16; ++ks)
+                    umma_bf16_ts(tO, tS + 32 + ks * 8, dV + ks * (HALVES * 2048 / 16), idO, 1u);
+                } else {
+#pragma unroll 1
+                  for (int ks = PA_BN / 32; ks < last_steps; ++ks)
+                    umma_bf16_ts(tO, tS + 32 + ks * 8, dV + ks * (HALVES * 2048 / 16), idO, 1u);
+                }
+                umma_commit(&sh.bar_empty[at_v]);
+                if (!has_next) break;
+                s_half(at, 1);
+                umma_commit(&sh.bar_empty[at]);
+                if (k + 2 * step >= nblk && pair) {
+                  umma_commit(&sh.bar_q_empty[qs]);
+                  umma_commit(&sh.bar_q_empty[qs]);
+                }
               }
-              if (!few && (pair ? v + 2 >= steps : v + 1 == steps)) umma_commit(&sh.bar_q_empty[qs]);
+              if (ok) umma_commit(&sh.bar_o[s]);
+            }
+          }
+          // loads of the other stream that are left
+          for (; ok && pos < 2 * nblk; ++pos) {
+            ok = mbar_wait(&sh.bar_full[st], ph);
+            mbar_arrive(&sh.bar_empty[st]);
+            if (++st == ST) {
+              st = 0;
+              ph ^= 1;
             }
           }
           if (!ok) break;
-          nq += pair ? 2 : 1;
-          const int loads = (2 * nblk) % (2 * ST);  // two turns of the ring keep the parity
-          for (int i = 0; i < loads; i += 2) advance(st0, ph0, 2);
         }
         // nothing may be in flight when the CTA gives back its TMEM
-        umma_commit(&sh.bar_end);
-        mbar_wait(&sh.bar_end, 0);
+        umma_commit(&sh.bar_end[s]);
+        mbar_wait(&sh.bar_end[s], 0);
       }
       __syncwarp();
-    } else if (warp == 11) {
-      // ---------------- clears the V rows of a tail that no query sees ----------------
-      // (up to the multiple of 16 at which the products stop)
-      uint32_t npiece = 0, ld0 = 0, nfix = 0;
-      PagedPiece piece;
-      while (next_piece(npiece, piece)) {
-        const int nblk = piece.nblk, last = piece.limit - (piece.j0 + nblk - 1) * PA_BN;
-        ld0 += 2 * nblk;
-        if (last >= PA_BN || (last & 15) == 0) continue;
-        if (!__all_sync(0xffffffffu, mbar_wait(&sh.bar_tail, nfix++ & 1))) break;  // the MMA thread has it
-        uint8_t* sV = sKV + ((ld0 - 1) % ST) * Tile::kv_bytes;                     // the piece's last load
-        for (int i = lane; i < (16 - (last & 15)) * HALVES * 8; i += 32) {
-          const int r = last + i / (HALVES * 8), ch = i % (HALVES * 8);
-          *reinterpret_cast<uint4*>(sV + (r >> 3) * (HALVES * 1024) + (ch >> 3) * 1024 + (r & 7) * 128 +
-                                    (ch & 7) * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.bar_fix);
-      }
-    } else if (warp == 10) {
+    } else {
       // ---------------- scheduler: the pieces of this CTA's share ----------------
       // Costs of the requests, 32 at a time, a request per lane (one of several
       // items is summed by the whole warp): once for their total, and again for
