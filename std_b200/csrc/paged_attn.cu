@@ -881,6 +881,18 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const int32_t* row = p.table + static_cast<size_t>(piece.b) * p.width;
         const int nblk = piece.nblk, limit = piece.limit;
         const bool pair = piece.tokens > p.TQ, few = piece.tokens <= p.TQ_few;
+        // the page of copy `lane` of block j (the copies of one page share it)
+        auto page_of = [&](int j) -> int {
+          const int key = j * PA_BN + lane * box;
+          if (lane >= per_block || j >= piece.j0 + nblk || key >= limit) return 0;
+          const int id = __ldg(row + (key >> p.page_log2));
+          if (id < 0 || id >= p.num_pages) {
+            std_set_error(STD_DEVERR_BOUNDS);
+            return p.num_pages;  // past the pool: TMA fills zeros
+          }
+          return id;
+        };
+        int next_id = page_of(piece.j0);
         // queries; a whole tile may take its slot's last half only when the few-row
         // piece before it is done there
         if (was_few && !few) ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_q_empty[(nq - 1) & 1], ((nq - 1) >> 1) & 1));
@@ -895,19 +907,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                           0, piece.h, piece.token0 + s * p.TQ);
           }
         }
-        // the page of copy `lane` of block j (the copies of one page share it)
-        auto page_of = [&](int j) -> int {
-          const int key = j * PA_BN + lane * box;
-          if (lane >= per_block || j >= piece.j0 + nblk || key >= limit) return 0;
-          const int id = __ldg(row + (key >> p.page_log2));
-          if (id < 0 || id >= p.num_pages) {
-            std_set_error(STD_DEVERR_BOUNDS);
-            return p.num_pages;  // past the pool: TMA fills zeros
-          }
-          return id;
-        };
-        // pair: K0 V0 K1 V1 ..; single (its streams start on two blocks): K0 K1 V0 K2 V1 .. V
-        int next_id = page_of(piece.j0), id = 0, id_before = 0, kk = 0, kv = 0;  // kk, kv: blocks of K, V so far
+        int id = 0, id_before = 0, kk = 0, kv = 0;  // kk, kv: blocks of K, V so far
 #pragma unroll 1
         for (int c = 0; ok && c < 2 * nblk; ++c) {
           const bool is_k = kk < nblk && (pair ? kk == kv : kk < kv + 2);
@@ -1247,104 +1247,145 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   }
 }
 
-// Joins the pieces of the items that cuts divide: block x looks at the item
+// Joins the pieces of the items that cuts divide: blocks x look at the item
 // that CTA x's share ends inside.  out = sum_c w_c o_c / sum_c w_c l_c with w_c =
-// exp2(m_c - max m), in a fixed order of the pieces.
+// exp2(m_c - max m), in a fixed order of the pieces.  Latency is what counts (a
+// few loads per row, mostly from L2): the grid is one wave, since each wave of
+// blocks costs a memory round trip even where there is nothing to join, and the
+// loads of two rows by two pieces a warp are in flight together, or, for an item
+// of many pieces (a long context), a row's pieces over eight warps.
+constexpr int PM_THREADS = 512, PM_Y = 2;  // (two blocks per SM)
+template <int D>
+struct PagedSum {  // a row's running (m, l, o)
+  float m, l, o[D / 32];
+  STD_DEV PagedSum() : m(-INFINITY), l(0.f) {
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) o[k] = 0.f;
+  }
+  // N pieces at once; one in which the row sees no key has l = 0, m = -inf, o = 0
+  template <int N>
+  STD_DEV void add(const float2 (&ml)[N], const float (&po)[N][D / 32]) {
+    float mx = m;
+#pragma unroll
+    for (int j = 0; j < N; ++j) mx = fmaxf(mx, ml[j].x);
+    const float a = l != 0.f ? exp2f(m - mx) : 0.f;
+    l *= a;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) o[k] *= a;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float w = ml[j].y != 0.f ? exp2f(ml[j].x - mx) : 0.f;
+      l += w * ml[j].y;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) o[k] += w * po[j][k];
+    }
+    m = mx;
+  }
+};
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(PM_THREADS, 2) paged_merge_kernel(const PagedAttnParams p) {
   pdl_launch_dependents();
   pdl_wait();
+  constexpr int PER = D / 32;  // columns per lane
   const int cta = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedSplit sp = p.splits[cta];
   if (sp.last_cta <= cta) return;
   const int n = sp.last_cta - cta + 1;
-  constexpr int PER = D / 32;  // columns per lane
-  constexpr int BATCH = 8;
-  // Few pieces: a warp per row.  Many (long contexts split over many CTAs): the
-  // block's eight warps share a row's pieces, so that their loads are in flight
-  // together, and add up in warp order.
-  const bool shared = n > BATCH;
-  const int parts = shared ? 8 : 1, part = shared ? warp : 0;
-  __shared__ float s_acc[8][D], s_l[8], s_m[8];
-  const int r_first = shared ? blockIdx.y : blockIdx.y * 8 + warp, r_step = shared ? gridDim.y : gridDim.y * 8;
-  for (int r = r_first; r < 256; r += r_step) {
-    const int rt = (r & 127) / p.G, t = (r >> 7) * p.TQ + rt;
-    if (rt >= p.TQ || t >= sp.tokens) continue;
-    // piece i is CTA cta + i's: its continued item (slot 0), or for the first the item begun there (slot 1)
-    const size_t row0 = static_cast<size_t>(2 * cta) * 256 + r;
-    auto at = [&](int i) { return row0 + static_cast<size_t>(2 * i + (i == 0 ? 1 : 0)) * 256; };
-    float m = -INFINITY, l = 0.f, acc[PER];
+  // piece i is CTA cta + i's: its continued item (slot 0), or for the first the item begun there (slot 1)
+  auto slot = [&](int i) { return (static_cast<size_t>(2 * (cta + i)) + (i == 0 ? 1 : 0)) * 256; };
+  auto load = [&](size_t row, bool there, float2& ml, float* o) {
+    ml = make_float2(-INFINITY, 0.f);
 #pragma unroll
-    for (int k = 0; k < PER; ++k) acc[k] = 0.f;
-    for (int i0 = part; i0 < n; i0 += parts * BATCH) {
-      float2 ml[BATCH];
-      float o[BATCH][PER];
-      float mb = m;
-#pragma unroll
-      for (int j = 0; j < BATCH; ++j) {
-        const int i = i0 + j * parts;
-        ml[j] = make_float2(-INFINITY, 0.f);
-#pragma unroll
-        for (int k = 0; k < PER; ++k) o[j][k] = 0.f;
-        if (i < n) {
-          ml[j] = __ldcg(p.ws_ml + at(i));
-          const float* src = p.ws_o + at(i) * D + lane * PER;
-          if constexpr (PER == 4) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
-            o[j][0] = v.x, o[j][1] = v.y, o[j][2] = v.z, o[j][3] = v.w;
-          } else {
-            const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-            o[j][0] = v.x, o[j][1] = v.y;
-          }
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < BATCH; ++j) mb = fmaxf(mb, ml[j].x);
-      const float scale = l != 0.f ? exp2f(m - mb) : 0.f;
-      l = l != 0.f ? l * scale : 0.f;
-#pragma unroll
-      for (int k = 0; k < PER; ++k) acc[k] = l != 0.f ? acc[k] * scale : 0.f;
-      m = mb;
-#pragma unroll
-      for (int j = 0; j < BATCH; ++j) {
-        if (ml[j].y == 0.f) continue;  // a piece in which the row sees no key
-        const float w = exp2f(ml[j].x - m);
-        l += w * ml[j].y;
-#pragma unroll
-        for (int k = 0; k < PER; ++k) acc[k] += w * o[j][k];
-      }
+    for (int k = 0; k < PER; ++k) o[k] = 0.f;
+    if (!there) return;
+    ml = __ldcg(p.ws_ml + row);
+    const float* src = p.ws_o + row * D + lane * PER;
+    if constexpr (PER == 4) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+      o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w;
+    } else {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+      o[0] = v.x, o[1] = v.y;
     }
-    if (shared) {
-#pragma unroll
-      for (int k = 0; k < PER; ++k) s_acc[warp][lane * PER + k] = acc[k];
-      if (lane == 0) s_l[warp] = l, s_m[warp] = m;
-      __syncthreads();
-      if (warp == 0) {
-        for (int w = 0; w < 8; ++w) m = fmaxf(m, s_m[w]);
-        l = 0.f;
-#pragma unroll
-        for (int k = 0; k < PER; ++k) acc[k] = 0.f;
-        for (int w = 0; w < 8; ++w) {
-          if (s_l[w] == 0.f) continue;
-          const float f = exp2f(s_m[w] - m);
-          l += f * s_l[w];
-#pragma unroll
-          for (int k = 0; k < PER; ++k) acc[k] += f * s_acc[w][lane * PER + k];
-        }
-      }
-      __syncthreads();  // before the next row's values
-      if (warp != 0) continue;
-    }
-    const float inv = l != 0.f ? 1.f / l : 0.f;
+  };
+  // rows: tile 0's from 0, tile 1's from 128
+  const int rows0 = min(sp.tokens, p.TQ) * p.G, rows1 = (sp.tokens - min(sp.tokens, p.TQ)) * p.G;
+  const int end = rows1 > 0 ? 128 + rows1 : rows0;
+  auto row_there = [&](int r) { return r < 128 ? r < rows0 : r - 128 < rows1; };
+  auto write = [&](int r, const PagedSum<D>& a) {
+    const float inv = a.l != 0.f ? 1.f / a.l : 0.f;
+    const int t = (r >> 7) * p.TQ + (r & 127) / p.G;
     const size_t orow = static_cast<size_t>(sp.token0 + t) * p.Hq + sp.kvh * p.G + (r & 127) % p.G;
     T* dst = static_cast<T*>(p.out) + orow * D + lane * PER;
     if constexpr (PER == 4)
       *reinterpret_cast<uint2*>(dst) =
-          make_uint2(pack_pair<T>(acc[0] * inv, acc[1] * inv), pack_pair<T>(acc[2] * inv, acc[3] * inv));
+          make_uint2(pack_pair<T>(a.o[0] * inv, a.o[1] * inv), pack_pair<T>(a.o[2] * inv, a.o[3] * inv));
     else
-      *reinterpret_cast<uint32_t*>(dst) = pack_pair<T>(acc[0] * inv, acc[1] * inv);
+      *reinterpret_cast<uint32_t*>(dst) = pack_pair<T>(a.o[0] * inv, a.o[1] * inv);
     if (lane == 0 && p.lse != nullptr)
-      p.lse[orow] = l != 0.f ? (m + log2f(l)) * 0.69314718055994530942f : -INFINITY;
+      p.lse[orow] = a.l != 0.f ? (a.m + log2f(a.l)) * 0.69314718055994530942f : -INFINITY;
+  };
+  if (n <= 8) {
+    constexpr int ROWS = 2, WARPS = PM_THREADS / 32;
+    for (int r0 = (blockIdx.y * WARPS + warp) * ROWS; r0 < end; r0 += PM_Y * WARPS * ROWS) {
+      bool there[ROWS];
+      PagedSum<D> sum[ROWS];
+#pragma unroll
+      for (int q = 0; q < ROWS; ++q) there[q] = row_there(r0 + q);
+      for (int i = 0; i < n; i += 2) {
+        float2 ml[ROWS][2];
+        float o[ROWS][2][PER];
+#pragma unroll
+        for (int q = 0; q < ROWS; ++q) {
+          load(slot(i) + r0 + q, there[q], ml[q][0], o[q][0]);
+          load(slot(i + 1) + r0 + q, there[q] && i + 1 < n, ml[q][1], o[q][1]);
+        }
+#pragma unroll
+        for (int q = 0; q < ROWS; ++q) sum[q].template add<2>(ml[q], o[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < ROWS; ++q)
+        if (there[q]) write(r0 + q, sum[q]);
+    }
+    return;
+  }
+  constexpr int ROWS = PM_THREADS / 256;  // rows at a time, eight warps each
+  __shared__ float s_o[ROWS][8][D];
+  __shared__ float2 s_ml[ROWS][8];
+  const int q = warp >> 3, part = warp & 7;
+  for (int r0 = blockIdx.y * ROWS; r0 < end; r0 += PM_Y * ROWS) {
+    const int r = r0 + q;
+    const bool there = row_there(r);
+    if (!__syncthreads_or(there ? 1 : 0)) continue;  // (and the last rows' values have been read)
+    PagedSum<D> sum;
+    for (int i0 = part; i0 < n; i0 += 32) {
+      float2 ml[4];
+      float o[4][PER];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) load(slot(i0 + 8 * j) + r, there && i0 + 8 * j < n, ml[j], o[j]);
+      sum.template add<4>(ml, o);
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k) s_o[q][part][lane * PER + k] = sum.o[k];
+    if (lane == 0) s_ml[q][part] = make_float2(sum.m, sum.l);
+    __syncthreads();
+    if (part == 0 && there) {
+      PagedSum<D> all;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float2 ml[4];
+        float o[4][PER];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          ml[w] = s_ml[q][4 * h + w];
+#pragma unroll
+          for (int k = 0; k < PER; ++k) o[w][k] = s_o[q][4 * h + w][lane * PER + k];
+        }
+        all.template add<4>(ml, o);
+      }
+      write(r, all);
+    }
   }
 }
 
@@ -1384,10 +1425,8 @@ static int paged_attn_launch(const CUtensorMap& tq, const CUtensorMap& tqf, cons
   if (launch_pdl(stdb::paged_attn_kernel<T, D>, dim3(stdb::PA_CTAS), dim3(stdb::PA_THREADS), stdb::PagedTile<D>::smem,
                  s, tq, tqf, tk, tv, p) != cudaSuccess)
     return 4;
-  // rows that an item can have: all of a pair's 256, or those of all the tokens there are
-  const int rows = p.T > p.TQ ? 256 : p.T * p.G;
-  const dim3 mgrid(stdb::PA_CTAS, rows < 8 ? rows : 8);
-  if (launch_pdl(stdb::paged_merge_kernel<T, D>, mgrid, dim3(256), 0, s, p) != cudaSuccess) return 4;
+  const dim3 mgrid(stdb::PA_CTAS, stdb::PM_Y);
+  if (launch_pdl(stdb::paged_merge_kernel<T, D>, mgrid, dim3(stdb::PM_THREADS), 0, s, p) != cudaSuccess) return 4;
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
 
