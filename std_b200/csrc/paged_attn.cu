@@ -1254,7 +1254,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 // blocks costs a memory round trip even where there is nothing to join, and the
 // loads of two rows by two pieces a warp are in flight together, or, for an item
 // of many pieces (a long context), a row's pieces over eight warps.
-constexpr int PM_THREADS = 512, PM_Y = 2;  // (two blocks per SM)
+constexpr int PM_THREADS = 512;  // (two blocks per SM)
 template <int D>
 struct PagedSum {  // a row's running (m, l, o)
   float m, l, o[D / 32];
@@ -1328,7 +1328,7 @@ __global__ void __launch_bounds__(PM_THREADS, 2) paged_merge_kernel(const PagedA
   };
   if (n <= 8) {
     constexpr int ROWS = 2, WARPS = PM_THREADS / 32;
-    for (int r0 = (blockIdx.y * WARPS + warp) * ROWS; r0 < end; r0 += PM_Y * WARPS * ROWS) {
+    for (int r0 = (blockIdx.y * WARPS + warp) * ROWS; r0 < end; r0 += gridDim.y * WARPS * ROWS) {
       bool there[ROWS];
       PagedSum<D> sum[ROWS];
 #pragma unroll
@@ -1354,7 +1354,7 @@ __global__ void __launch_bounds__(PM_THREADS, 2) paged_merge_kernel(const PagedA
   __shared__ float s_o[ROWS][8][D];
   __shared__ float2 s_ml[ROWS][8];
   const int q = warp >> 3, part = warp & 7;
-  for (int r0 = blockIdx.y * ROWS; r0 < end; r0 += PM_Y * ROWS) {
+  for (int r0 = blockIdx.y * ROWS; r0 < end; r0 += gridDim.y * ROWS) {
     const int r = r0 + q;
     const bool there = row_there(r);
     if (!__syncthreads_or(there ? 1 : 0)) continue;  // (and the last rows' values have been read)
@@ -1425,7 +1425,7 @@ static int paged_attn_launch(const CUtensorMap& tq, const CUtensorMap& tqf, cons
   if (launch_pdl(stdb::paged_attn_kernel<T, D>, dim3(stdb::PA_CTAS), dim3(stdb::PA_THREADS), stdb::PagedTile<D>::smem,
                  s, tq, tqf, tk, tv, p) != cudaSuccess)
     return 4;
-  const dim3 mgrid(stdb::PA_CTAS, stdb::PM_Y);
+  const dim3 mgrid(stdb::PA_CTAS, p.T > p.TQ ? 4 : 2);
   if (launch_pdl(stdb::paged_merge_kernel<T, D>, mgrid, dim3(stdb::PM_THREADS), 0, s, p) != cudaSuccess) return 4;
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }
