@@ -58,6 +58,7 @@ constexpr float PA_RESCALE = 8.0f;  // log2 units
 // Cost of a block in a single and in a pair; an item costs PA_OVER blocks more
 // (its queries, first keys and output).
 constexpr int PA_W1 = 2, PA_W2 = 3, PA_OVER = 2;
+constexpr int PA_WHOLE = 4;  // an item of at most this many blocks is not divided: it goes where it begins
 
 // Shared memory: two query slots and a ring of K/V blocks.  A slot holds a
 // 128-row Q tile (halves of 64 columns, 16 KB apart), or, for few rows, a 64-row
@@ -179,8 +180,8 @@ struct PagedWalk {
       paged_item(p, n, kv, i, t0, nt, limit, nb, w);
       const int cost = paged_item_cost(p, n, kv, i);
       const int end = min(cost, skip + rem);
-      j0 = paged_cut(p, skip, w);
-      j1 = min(nb, paged_cut(p, end, w));
+      j0 = nb <= PA_WHOLE ? (skip > 0 ? nb : 0) : paged_cut(p, skip, w);
+      j1 = nb <= PA_WHOLE ? nb : min(nb, paged_cut(p, end, w));
       rem -= end - skip;
       skip = 0;
       cut = end;
@@ -884,14 +885,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         // the page of copy `lane` of block j (the copies of one page share it)
         auto page_of = [&](int j) -> int {
           const int key = j * PA_BN + lane * box;
-          if (lane >= per_block || j >= piece.j0 + nblk || key >= limit) return 0;
-          const int id = __ldg(row + (key >> p.page_log2));
-          if (id < 0 || id >= p.num_pages) {
-            std_set_error(STD_DEVERR_BOUNDS);
-            return p.num_pages;  // past the pool: TMA fills zeros
-          }
-          return id;
-        };
+          return lane < per_block && j < piece.j0 + nblk && key < limit ? __ldg(row + (key >> p.page_log2)) : 0;
+        };  // (not looked at before it is used: the load is on its way meanwhile)
         int next_id = page_of(piece.j0);
         // queries; a whole tile may take its slot's last half only when the few-row
         // piece before it is done there
@@ -927,9 +922,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           __syncwarp();
           if (lane < copies) {
             const int key = j * PA_BN + lane * box;
-            const int g = (mine * p.Hkv + piece.h) * groups + ((key & ((1 << p.page_log2) - 1)) >> 3);
+            const bool in_pool = mine >= 0 && mine < p.num_pages;
+            if (!in_pool) std_set_error(STD_DEVERR_BOUNDS);
+            const int g = ((in_pool ? mine : 0) * p.Hkv + piece.h) * groups + ((key & ((1 << p.page_log2) - 1)) >> 3);
             tma_load_4d(sKV + st * Tile::kv_bytes + lane * copy_bytes, is_k ? &tmK : &tmV, &sh.bar_full[st], 0, 0, 0,
-                        mine >= p.num_pages ? p.num_pages * p.Hkv * groups : g);
+                        in_pool ? g : p.num_pages * p.Hkv * groups);  // (past the pool: TMA fills zeros)
           }
           ++nld;
           if (is_k)
@@ -1142,31 +1139,33 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       // instructions come from L2, and short code is what makes this quick.)
       PagedWalk walk;
       walk.rem = 0;
-      int total = 0, share = 1, x0 = 0, off = 0;
+      int total = 0, share = 1, x0 = 0, off = 0, cost = 0;
 #pragma unroll 1
       for (int pass = 0; pass < 2; ++pass) {
         int run = 0;
 #pragma unroll 1
         for (int b0 = 0; b0 < p.B; b0 += 32) {
-          const int b = b0 + lane;
-          int n = 0, kv = 0;
-          if (b < p.B) {
-            kv = __ldg(p.kv_lens + b);
-            if (!paged_request(p, __ldg(p.cu_q + b), __ldg(p.cu_q + b + 1), kv, n) && cta == 0)
-              std_set_error(STD_DEVERR_LENGTH);
-          }
-          int cost = n > 0 && n <= 2 * p.TQ ? paged_item_cost(p, n, kv, 0) : 0;
+          if (pass == 0 || p.B > 32) {  // (else `cost` still is what pass 0 left)
+            const int b = b0 + lane;
+            int n = 0, kv = 0;
+            if (b < p.B) {
+              kv = __ldg(p.kv_lens + b);
+              if (!paged_request(p, __ldg(p.cu_q + b), __ldg(p.cu_q + b + 1), kv, n) && cta == 0)
+                std_set_error(STD_DEVERR_LENGTH);
+            }
+            cost = n > 0 && n <= 2 * p.TQ ? paged_item_cost(p, n, kv, 0) : 0;
 #pragma unroll 1
-          for (uint32_t many = __ballot_sync(0xffffffffu, n > 2 * p.TQ); many != 0; many &= many - 1) {
-            const int src = __ffs(many) - 1;
-            const int n_ = __shfl_sync(0xffffffffu, n, src), kv_ = __shfl_sync(0xffffffffu, kv, src);
-            int sum = 0;
+            for (uint32_t many = __ballot_sync(0xffffffffu, n > 2 * p.TQ); many != 0; many &= many - 1) {
+              const int src = __ffs(many) - 1;
+              const int n_ = __shfl_sync(0xffffffffu, n, src), kv_ = __shfl_sync(0xffffffffu, kv, src);
+              int sum = 0;
 #pragma unroll 1
-            for (int i = lane; i * 2 * p.TQ < n_; i += 32) sum += paged_item_cost(p, n_, kv_, i);
-            sum = __reduce_add_sync(0xffffffffu, sum);
-            if (lane == src) cost = sum;
+              for (int i = lane; i * 2 * p.TQ < n_; i += 32) sum += paged_item_cost(p, n_, kv_, i);
+              sum = __reduce_add_sync(0xffffffffu, sum);
+              if (lane == src) cost = sum;
+            }
+            cost *= p.Hkv;
           }
-          cost *= p.Hkv;
           if (pass == 0) {
             total += __reduce_add_sync(0xffffffffu, cost);
             continue;
@@ -1192,22 +1191,29 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       if (walk.rem > 0) {
         walk.request(p);
         // KV head and item: the items' costs, a run of `per` of them per lane
-        const int per = (walk.items + 31) / 32;
-        int sum = 0;
+        if (walk.items == 1) {
+          const int head = paged_item_cost(p, walk.n, walk.kv, 0);
+          walk.h = off / head;
+          walk.i = 0;
+          walk.skip = off - walk.h * head;
+        } else {
+          const int per = (walk.items + 31) / 32;
+          int sum = 0;
 #pragma unroll 1
-        for (int i = lane * per; i < min((lane + 1) * per, walk.items); ++i) sum += paged_item_cost(p, walk.n, walk.kv, i);
-        const int inc = warp_scan(sum, lane), head = __shfl_sync(0xffffffffu, inc, 31);
-        walk.h = off / head;
-        off -= walk.h * head;
-        const int src = __ffs(__ballot_sync(0xffffffffu, off < inc)) - 1;
-        off -= __shfl_sync(0xffffffffu, inc - sum, src);
+          for (int i = lane * per; i < min((lane + 1) * per, walk.items); ++i) sum += paged_item_cost(p, walk.n, walk.kv, i);
+          const int inc = warp_scan(sum, lane), head = __shfl_sync(0xffffffffu, inc, 31);
+          walk.h = off / head;
+          off -= walk.h * head;
+          const int src = __ffs(__ballot_sync(0xffffffffu, off < inc)) - 1;
+          off -= __shfl_sync(0xffffffffu, inc - sum, src);
 #pragma unroll 1
-        for (walk.i = src * per;; ++walk.i) {
-          const int c = paged_item_cost(p, walk.n, walk.kv, walk.i);
-          if (off < c || walk.i + 1 >= walk.items) break;
-          off -= c;
+          for (walk.i = src * per;; ++walk.i) {
+            const int c = paged_item_cost(p, walk.n, walk.kv, walk.i);
+            if (off < c || walk.i + 1 >= walk.items) break;
+            off -= c;
+          }
+          walk.skip = off;
         }
-        walk.skip = off;
       }
       PagedSplit split = {-1, 0, 0, 0};
       bool more = true;
@@ -1425,6 +1431,9 @@ static int paged_attn_launch(const CUtensorMap& tq, const CUtensorMap& tqf, cons
   if (launch_pdl(stdb::paged_attn_kernel<T, D>, dim3(stdb::PA_CTAS), dim3(stdb::PA_THREADS), stdb::PagedTile<D>::smem,
                  s, tq, tqf, tk, tv, p) != cudaSuccess)
     return 4;
+  // nothing to join where no item is long enough to be divided
+  if (static_cast<long long>(p.width) << p.page_log2 <= stdb::PA_WHOLE * stdb::PA_BN)
+    return cudaGetLastError() == cudaSuccess ? 0 : 4;
   const dim3 mgrid(stdb::PA_CTAS, p.T > p.TQ ? 4 : 2);
   if (launch_pdl(stdb::paged_merge_kernel<T, D>, mgrid, dim3(stdb::PM_THREADS), 0, s, p) != cudaSuccess) return 4;
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
@@ -1457,12 +1466,14 @@ extern "C" int std_paged_attn(const void* q, const void* k_pages, const void* v_
                             static_cast<uint64_t>(T)};
     const uint64_t qs[3] = {row, row * G, row * Hq};
     const uint32_t qb[4] = {64, static_cast<uint32_t>(G), 1, static_cast<uint32_t>(TQ)};
-    int rc = paged_tmap_4d(&tq, is_fp16, q, qd, qs, qb);
+    // (one of the two maps is never used where no item, or every item, has few rows)
+    int rc = T > TQ_few ? paged_tmap_4d(&tq, is_fp16, q, qd, qs, qb) : 0;
     if (rc != 0) return rc;
-    // (heads in groups of more than 64 have no few-row items: the map is not used)
-    const uint32_t qfb[4] = {64, static_cast<uint32_t>(G), 1, static_cast<uint32_t>(TQ_few > 0 ? TQ_few : 1)};
-    rc = paged_tmap_4d(&tqf, is_fp16, q, qd, qs, qfb);
+    const uint32_t qfb[4] = {64, static_cast<uint32_t>(G), 1, static_cast<uint32_t>(TQ_few)};
+    if (TQ_few > 0) rc = paged_tmap_4d(&tqf, is_fp16, q, qd, qs, qfb);
     if (rc != 0) return rc;
+    if (T <= TQ_few) tq = tqf;
+    if (TQ_few == 0) tqf = tq;
     const uint64_t kd[4] = {64, 8, static_cast<uint64_t>(D / 64),
                             static_cast<uint64_t>(num_pages) * Hkv * (page_size / 8)};
     const uint64_t ks[3] = {row, 128, row * 8};
