@@ -18,8 +18,12 @@ _WS: Dict[Tuple[str, int], torch.Tensor] = {}
 
 
 def _stream() -> int:
-    # the raw handle of torch.cuda.current_stream(), without building a Stream object (3 us a call)
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return _stream_of(torch.cuda.current_device())
+
+
+def _stream_of(device: int) -> int:
+    # the raw handle of torch.cuda.current_stream(device), without building a Stream object (3 us a call)
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _p(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -380,6 +384,7 @@ def argmax_rows(logits: torch.Tensor, out: torch.Tensor, n: int = 1, out_stride:
 # ----------------------------------------------------------------------------
 
 _PAGED_DTYPES = (torch.bfloat16, torch.float16)
+_PAGED_WS_BYTES: Dict[int, int] = {}
 
 
 def _paged_check(dtype: torch.dtype, device: int, *tensors) -> None:
@@ -454,7 +459,7 @@ def paged_update(past_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
     _lib.call("std_paged_update", past_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
               n_blocks.data_ptr(), free_pages.data_ptr(), n_free.data_ptr(), B, width, int(page_size), num_pages,
               max_tokens, cu_q.data_ptr(), kv_lens.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-              admitted.data_ptr(), _stream())
+              admitted.data_ptr(), _stream_of(device))
     return cu_q, kv_lens, slots, positions, admitted
 
 
@@ -478,7 +483,7 @@ def paged_rope_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.T
     _paged_check(torch.int32, device, (positions, "positions", (T,)), (slots, "slots", (T,)))
     _lib.call("std_paged_rope_append", qkv.data_ptr(), T, Hq, Hkv, D, 1 if dtype == torch.float16 else 0,
               positions.data_ptr(), slots.data_ptr(), cos_t.data_ptr(), sin_t.data_ptr(), max_pos, q_out.data_ptr(),
-              k_pages.data_ptr(), v_pages.data_ptr(), num_pages, page, _stream())
+              k_pages.data_ptr(), v_pages.data_ptr(), num_pages, page, _stream_of(device))
     return q_out
 
 
@@ -519,10 +524,13 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         _paged_check(torch.float32, device, (lse, "lse", (T, Hq)))
     # Of this call alone: the caching allocator hands it out in stream order, and
     # under capture from the graph's own pool, so no two calls or graphs share it.
-    ws = torch.empty(_lib.query("std_paged_attn_workspace_bytes", D), dtype=torch.uint8, device=q.device)
+    nb = _PAGED_WS_BYTES.get(D)
+    if nb is None:
+        nb = _PAGED_WS_BYTES[D] = _lib.query("std_paged_attn_workspace_bytes", D)
+    ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
     _lib.call("std_paged_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
               cu_q.data_ptr(), kv_lens.data_ptr(), T, B, Hq, Hkv, D, 1 if dtype == torch.float16 else 0, num_pages,
-              page, width, 1 if causal else 0, scale, out.data_ptr(), _p(lse), ws.data_ptr(), ws.numel(), _stream())
+              page, width, 1 if causal else 0, scale, out.data_ptr(), _p(lse), ws.data_ptr(), nb, _stream_of(device))
     return out
 
 
