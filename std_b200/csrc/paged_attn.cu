@@ -20,9 +20,9 @@
 // is raised lazily, when a block passes it by more than 2^8, so O is normally
 // not touched between blocks.
 //
-// Few rows.  A single item of at most 64 rows (decoding: G rows) is computed
+// Few rows.  A single item of at most 32 rows (decoding: G rows) is computed
 // transposed, keys on the 128 MMA rows and the query rows on N:
-//   S^T = K Q^T    M=128 (keys) N=16 or 64, both operands in shared memory
+//   S^T = K Q^T    M=128 (keys) N=16 or 32, both operands in shared memory
 //   O^T += V^T P^T M=128 (head dims), A = V MN-major, B = P^T in shared memory
 // A softmax thread then owns one key and N rows, so a block costs N exponentials
 // a thread on all 128 threads instead of 128 on the few threads that have a row,
@@ -61,7 +61,7 @@ constexpr int PA_W1 = 2, PA_W2 = 3, PA_OVER = 2;
 constexpr int PA_WHOLE = 4;  // an item of at most this many blocks is not divided: it goes where it begins
 
 // Shared memory: two query slots and a ring of K/V blocks.  A slot holds a
-// 128-row Q tile (halves of 64 columns, 16 KB apart), or, for few rows, a 64-row
+// 128-row Q tile (halves of 64 columns, 16 KB apart), or, for few rows, a 32-row
 // one (halves 8 KB apart) in its first 16 KB and P^T of stream = slot (a 128-byte
 // row per key) in its last 16 KB.
 constexpr uint32_t PA_SLOT = 32768, PA_PT = 16384;
@@ -71,7 +71,7 @@ struct PagedTile {
   static constexpr int stages = D == 128 ? 5 : 8;
   static constexpr uint32_t smem = 2 * PA_SLOT + stages * kv_bytes + 1024;
 };
-constexpr int PA_FEW = 64;  // most rows of an item that is computed transposed
+constexpr int PA_FEW = 32;  // most rows of an item that is computed transposed
 constexpr int PA_POLY = 4;  // every 4th pair of exponentials on the FMA pipe
 
 // What a CTA leaves for the merge about the item that its share ends inside.
@@ -86,7 +86,7 @@ struct PagedAttnParams {
   const int32_t* table;  // [B, width]
   const int32_t* cu_q;   // [B + 1]
   const int32_t* kv_lens;
-  int T, B, width, page_log2, num_pages, Hq, Hkv, G, TQ, TQ_few, causal;  // TQ_few = floor(64 / G)
+  int T, B, width, page_log2, num_pages, Hq, Hkv, G, TQ, TQ_few, causal;  // TQ_few = floor(32 / G)
   float scale_log2;
   void* out;   // [T, Hq, D]
   int out_32b;    // out is 32-byte aligned
@@ -199,7 +199,7 @@ __host__ __device__ constexpr uint32_t paged_idesc(int M, int N, int a_mn_major,
          (std::is_same<T, __half>::value ? ~((1u << 7) | (1u << 10)) : ~0u);
 }
 // MMA columns for `rows` few rows.
-STD_DEV int paged_few_cols(int rows) { return rows <= 16 ? 16 : 64; }
+STD_DEV int paged_few_cols(int rows) { return rows <= 16 ? 16 : 32; }
 
 STD_DEV void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z, int w) {
   asm volatile(
@@ -456,8 +456,8 @@ STD_DEV bool paged_softmax_half(uint32_t tS, uint32_t tO, float sc, int nvis, fl
   return true;
 }
 
-// Combines N values of each lane over the warp: halving the rows a lane keeps at
-// each step, max(1, N / 32) of them are left, rows `base` and up.
+// Combines N <= 32 values of each lane over the warp, halving the rows a lane keeps
+// at each step; row `base` is left.
 template <int N, typename Op>
 STD_DEV int warp_reduce_rows(float* v, int lane, Op op) {
   int base = 0;
@@ -541,7 +541,6 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
       for (int n = 0; n < N; ++n) v[n] = y[n];
       const int base = warp_reduce_rows<N>(v, lane, [](float a, float b) { return fmaxf(a, b); });
       red(s, w, base) = v[0];
-      if (N == 64) red(s, w, base + 1) = v[1];
       if (!group_sync()) return false;
       if (key < N) {
         const float mx = fmaxf(fmaxf(red(s, 0, key), red(s, 1, key)), fmaxf(red(s, 2, key), red(s, 3, key)));
@@ -593,7 +592,6 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
     if (!__all_sync(0xffffffffu, mbar_wait(&sh.bar_o[s], no++ & 1))) return false;
     const int base = warp_reduce_rows<N>(l, lane, [](float a, float b) { return a + b; });
     red(s, w, base) = l[0];
-    if (N == 64) red(s, w, base + 1) = l[1];
     fence_async_smem();  // (a TMA load may write here next)
   }
   if (s == 1) {
@@ -739,7 +737,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         if (rows <= 16)
           ok = paged_few_piece<T, D, 16>(p, piece, sh, sQ, sV, tS, tO, s, &sh.bar_q_empty[nq++ & 1], ntail, ns, no, nj, ng);
         else
-          ok = paged_few_piece<T, D, 64>(p, piece, sh, sQ, sV, tS, tO, s, &sh.bar_q_empty[nq++ & 1], ntail, ns, no, nj, ng);
+          ok = paged_few_piece<T, D, 32>(p, piece, sh, sQ, sV, tS, tO, s, &sh.bar_q_empty[nq++ & 1], ntail, ns, no, nj, ng);
         continue;
       }
       nq += pair ? 2 : 1;

@@ -138,6 +138,10 @@ CASES = [
     ([(9000, 1), (20, 1)], 8, 1, 128, 16, BF, True),
     ([(6000, 40)], 12, 2, 128, 64, BF, True),
     ([(5, 1300)], 40, 8, 64, 16, FP, True),
+    # rows of an item on both sides of 16, 32, 64 and 128, alone and beside each other
+    ([(700, 2), (90, 3), (1300, 4), (2, 5), (640, 9), (31, 10), (128, 18), (0, 1)], 28, 4, 128, 64, BF, True),
+    ([(2600, 1), (3, 2), (2000, 3), (900, 4), (77, 8)], 16, 1, 64, 16, FP, False),
+    ([(1500, 32), (20, 33), (1, 16), (600, 64), (130, 17), (9, 128)], 4, 4, 128, 32, FP, True),
 ]
 
 
