@@ -362,3 +362,271 @@ def test_append_reports_out_of_range(ops):
     ops.paged_rope_append(qkv, _i32([0, 9, 2]), _i32([-1, -1, -1]), cos, sin, last, k, v)
     assert torch.equal(last[1], q[1])  # read as the last position
     _no_device_error(ops)
+
+
+# ------------------------------------------------------------------ misuse, and odd use
+def test_attention_bad_entries_are_reported(ops):
+    """Page ids, lengths and token ranges that do not fit: reported, nothing read or
+    written out of range, the other requests right."""
+    x = Paged([(300, 4), (200, 30), (90, 1), (40, 50)], 28, 4, 128, 16, BF, seed=1)
+    good = x.call(ops)
+    x.check(good, None)
+    for bad in (-7, x.k.shape[0], 2 ** 30):
+        keep = x.table[0, 3].item()
+        x.table[0, 3] = bad
+        out = x.call(ops)
+        assert ops.device_error() == 2
+        assert torch.isfinite(out[:4]).all() and torch.equal(out[4:], good[4:])
+        x.table[0, 3] = keep
+    # (request 1 has 15 pages; a length cut to the table's width reaches the -1 behind them)
+    room = x.table.shape[1] * 16
+    table = torch.where(x.table < 0, 0, x.table)
+    for lens in ([304, -3, 91, 90], [304, room + 1, 91, 90], [304, 2 ** 31 - 1, 91, 90]):
+        out = torch.full_like(x.q, 3.0)
+        ops.paged_attention(x.q, x.k, x.v, table, x.cu, _i32(lens), out=out)
+        assert ops.device_error() == 3
+        assert torch.equal(out[:4], good[:4]) and torch.equal(out[34:35], good[34:35])
+    for cu in ([0, 4, 34, 35, 86], [0, 4, 2, 35, 85], [0, -4, 34, 35, 85], [-1, 4, 34, 35, 85]):
+        out = torch.full_like(x.q, 3.0)
+        ops.paged_attention(x.q, x.k, x.v, x.table, _i32(cu), x.kv_lens, out=out)
+        assert ops.device_error() == 3
+    out = torch.full_like(x.q, 3.0)
+    ops.paged_attention(x.q, x.k, x.v, x.table, _i32([0, 4, 34, 35, 86]), x.kv_lens, out=out)
+    assert ops.device_error() == 3
+    assert torch.equal(out[:35], good[:35]) and (out[35:] == 3).all()  # the last request skipped
+    _no_device_error(ops)
+
+
+def test_attention_no_tokens(ops):
+    x = Paged([(30, 0), (5, 0)], 28, 4, 128, 16, BF, tail_rows=4)
+    out = torch.full_like(x.q, 3.0)
+    x.call(ops, out=out)
+    assert (out == 3).all()
+    none = x.q[:0]
+    assert ops.paged_attention(none, x.k, x.v, x.table, x.cu, x.kv_lens).shape == (0, 28, 128)
+    _no_device_error(ops)
+
+
+def test_attention_shared_pages_and_order(ops):
+    """Requests that share their first pages, and the same request in other batches
+    and places: within rounding of one another."""
+    x = Paged([(1000, 3), (700, 40), (64, 1)], 28, 4, 128, 32, BF, seed=2)
+    out = x.call(ops)
+    x.check(out, None)
+    table = torch.stack([x.table[1], x.table[0], x.table[1]])
+    q = torch.cat([x.q[3:43], x.q[:3], x.q[3:43]])
+    o2 = ops.paged_attention(q, x.k, x.v, table, _i32([0, 40, 43, 83]), _i32([740, 1003, 740]))
+    x2 = Paged.__new__(Paged)
+    x2.__dict__.update(x.__dict__, pairs=[(700, 40), (1000, 3), (700, 40)], kv=[740, 1003, 740], q=q,
+                       keys=[x.keys[1], x.keys[0], x.keys[1]])
+    x2.check(o2, None)
+    _no_device_error(ops)
+
+
+def test_attention_offsets_beyond_32_bits(ops):
+    """Pools of more than 2^32 bytes and 2^31 elements, the pages used at their end and
+    their start."""
+    num_pages, Hkv, page, D = 70000, 4, 64, 128  # 2.3e9 elements a pool
+    k = torch.empty(num_pages, Hkv, page, D, dtype=BF, device="cuda")
+    v = torch.empty_like(k)
+    small = Paged([(500, 3), (100, 40)], 28, Hkv, D, page, BF, seed=8)
+    ids = [num_pages - 1 - 3 * i if i % 2 == 0 else i for i in range(small.k.shape[0])]
+    k[ids], v[ids] = small.k, small.v
+    table = torch.where(small.table >= 0, torch.tensor(ids, dtype=torch.int32, device="cuda")[small.table.clamp(min=0).long()],
+                        -1)
+    out = ops.paged_attention(small.q, k, v, table.int().contiguous(), small.cu, small.kv_lens)
+    assert torch.equal(out, small.call(ops))
+    cos, sin = _rope_tables(16, D, BF)
+    qkv = torch.randn(2, (28 + 2 * Hkv) * D, device="cuda").to(BF)
+    q = torch.empty(2, 28, D, dtype=BF, device="cuda")
+    ops.paged_rope_append(qkv, _i32([0, 0]), _i32([num_pages * page - 1, 5]), cos, sin, q, k, v)
+    want = qkv.view(2, -1, D)  # position 0: no rotation
+    assert torch.equal(k[-1, :, -1], want[0, 28:32]) and torch.equal(v[-1, :, -1], want[0, 32:])
+    assert torch.equal(k[0, :, 5], want[1, 28:32]) and torch.equal(q, want[:, :28])
+    _no_device_error(ops)
+
+
+def test_attention_scores_of_one_sign_and_infinities_behind_the_end(ops):
+    """Strongly negative scores everywhere (exponentials far below the first guess of
+    the maximum), and +-inf instead of NaN in the rows that no query may read."""
+    for dtype in (BF, FP):
+        x = Paged([(700, 1), (300, 50), (10, 9)], 8, 2, 128, 64, dtype, seed=4)
+        x.q = x.q.abs()
+        x.keys = [(-k.abs(), v) for k, v in x.keys]
+        for b, (kb, _) in enumerate(x.keys):
+            for i in range(-(-x.kv[b] // 64)):
+                rows = slice(i * 64, min(x.kv[b], (i + 1) * 64))
+                x.k[x.table[b, i].item(), :, :rows.stop - rows.start] = kb[rows].permute(1, 0, 2)
+        x.k = torch.where(x.k.isnan(), float("inf"), x.k).to(dtype)
+        x.v = torch.where(x.v.isnan(), float("-inf"), x.v).to(dtype)
+        lse = torch.empty(x.q.shape[:2], device="cuda")
+        x.check(x.call(ops, lse=lse), lse)
+    _no_device_error(ops)
+
+
+def test_two_streams_and_repeated_calls(ops):
+    """Calls on two streams at once do not disturb one another."""
+    a, b = Paged([(4000, 1), (3000, 3)], 28, 4, 128, 16, BF, seed=1), Paged([(100, 900)], 16, 16, 64, 32, FP, seed=2)
+    want_a, want_b = a.call(ops), b.call(ops)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got_a, got_b = [], []
+    for _ in range(8):
+        with torch.cuda.stream(s1):
+            got_a.append(a.call(ops))
+        with torch.cuda.stream(s2):
+            got_b.append(b.call(ops))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want_a) for g in got_a) and all(torch.equal(g, want_b) for g in got_b)
+    _no_device_error(ops)
+
+
+def test_wrapper_refusals(ops):
+    x = Paged([(30, 2)], 28, 4, 128, 16, BF)
+    with pytest.raises(RuntimeError, match="float32"):
+        ops.paged_attention(x.q.float(), x.k, x.v, x.table, x.cu, x.kv_lens)
+    with pytest.raises(RuntimeError, match="k_pages"):
+        ops.paged_attention(x.q.half(), x.k, x.v, x.table, x.cu, x.kv_lens)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        ops.paged_attention(x.q, x.k.transpose(1, 2).contiguous().transpose(1, 2), x.v, x.table, x.cu, x.kv_lens)
+    with pytest.raises(ValueError, match="v_pages"):
+        ops.paged_attention(x.q, x.k, x.v[:-1], x.table, x.cu, x.kv_lens)
+    with pytest.raises(ValueError, match="cu_q"):
+        ops.paged_attention(x.q, x.k, x.v, x.table, x.cu[:1], x.kv_lens)
+    with pytest.raises(ValueError, match="multiple"):
+        ops.paged_attention(x.q[:, :27].contiguous(), x.k, x.v, x.table, x.cu, x.kv_lens)
+    with pytest.raises(ValueError, match="scale"):
+        ops.paged_attention(x.q, x.k, x.v, x.table, x.cu, x.kv_lens, scale=0.0)
+    with pytest.raises(ValueError, match="page_size"):
+        ops.paged_attention(x.q, x.k[:, :, :8].contiguous(), x.v[:, :, :8].contiguous(), x.table, x.cu, x.kv_lens)
+    with pytest.raises(RuntimeError, match="status 1"):
+        ops.paged_attention(x.q, x.k, x.v, x.table, x.cu, x.kv_lens, out=x.q)
+    with pytest.raises(RuntimeError, match="int32"):
+        ops.paged_update(x.kv_lens.long(), x.kv_lens, x.table, x.kv_lens, x.kv_lens, x.kv_lens, 16, 4)
+    with pytest.raises(ValueError, match="n_free"):
+        ops.paged_update(x.kv_lens, x.kv_lens, x.table, x.kv_lens, x.kv_lens, x.cu, 16, 4)
+    with pytest.raises(RuntimeError, match="status 1"):
+        ops.paged_update(x.kv_lens, x.kv_lens, x.table, x.kv_lens, x.kv_lens, x.kv_lens, 24, 4)
+    _no_device_error(ops)
+
+
+# ------------------------------------------------------------------ together
+def _serve(ops, graph):
+    """A server's steps over one layer: prompts in chunks beside decoding requests,
+    drafts given up again, requests that end and make room, one that has to wait."""
+    Hq, Hkv, D, page, num_pages, width, B, rows = 28, 4, 128, 16, 40, 24, 4, 160
+    g = torch.Generator().manual_seed(9)
+    cos, sin = _rope_tables(width * page, D, BF)
+    k = torch.full((num_pages, Hkv, page, D), float("nan"), dtype=BF, device="cuda")
+    v = torch.full_like(k, float("nan"))
+    ids = list(range(num_pages))
+    random.Random(3).shuffle(ids)
+    table, n_blocks = torch.full((B, width), -1, dtype=torch.int32, device="cuda"), _i32([0] * B)
+    free, n_free = _i32(ids), _i32([num_pages])
+    past, new = _i32([0] * B), _i32([0] * B)
+    qkv = torch.zeros(rows, (Hq + 2 * Hkv) * D, dtype=BF, device="cuda")
+    q, out = torch.zeros(rows, Hq, D, dtype=BF, device="cuda"), torch.zeros(rows, Hq, D, dtype=BF, device="cuda")
+    step_out = tuple(torch.zeros(n, dtype=torch.int32, device="cuda") for n in (B + 1, B, rows, rows, B))
+
+    def run():
+        cu, kv_lens, slots, positions, _ = ops.paged_update(past, new, table, n_blocks, free, n_free, page, rows,
+                                                            out=step_out)
+        ops.paged_rope_append(qkv, positions, slots, cos, sin, q, k, v)
+        ops.paged_attention(q, k, v, table, cu, kv_lens, out=out)
+
+    run()  # nothing new: allocates and loads before the capture
+    if graph:
+        cg = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(cg):
+            run()
+    hist = [[] for _ in range(B)]  # each request's (rotated k, v) so far
+    e = torch.finfo(BF).eps
+    #        past lengths, new tokens, which are admitted
+    steps = [([0, 0, 0, 0], [100, 30, 7, 0], [1, 1, 1, 1]),
+             ([100, 30, 7, 0], [1, 10, 120, 0], [1, 1, 1, 1]),
+             ([101, 33, 127, 0], [1, 1, 1, 90], [1, 1, 1, 1]),        # 7 of 10 drafts given up
+             ([102, 34, 128, 90], [60, 70, 1, 20], [1, 1, 1, 1]),
+             ([162, 104, 129, 110], [100, 1, 1, 50], [1, 1, 1, 0]),   # the last one does not fit
+             ([0, 105, 130, 110], [0, 1, 1, 50], [1, 1, 1, 1])]       # the first one has ended
+    for past_l, new_l, admitted in steps:
+        past.copy_(_i32(past_l))
+        new.copy_(_i32(new_l))
+        x = torch.randn(rows, (Hq + 2 * Hkv) * D, generator=g).to(BF)
+        qkv.copy_(x)
+        out.fill_(9.0)
+        cg.replay() if graph else run()
+        assert step_out[4].tolist() == admitted
+        at = 0
+        for b, (p, n) in enumerate(zip(past_l, new_l)):
+            mine = x[at:at + n].view(n, Hq + 2 * Hkv, D).cuda()
+            if not admitted[b]:
+                assert (out[at:at + n] == 0).all()
+                at += n
+                continue
+            pos = torch.arange(p, p + n, device="cuda")
+            y = mine.double()
+            lo, hi = y[..., :D // 2], y[..., D // 2:]
+            c, s = cos[pos].double()[:, None], sin[pos].double()[:, None]
+            y = torch.cat([lo * c - hi * s, hi * c + lo * s], -1).to(BF)
+            hist[b] = hist[b][:p] + [(y[i, Hq:Hq + Hkv], mine[i, Hq + Hkv:]) for i in range(n)]
+            at += n
+            if n == 0:
+                continue
+            G = Hq // Hkv
+            kb = torch.stack([h[0] for h in hist[b]]).double().permute(1, 0, 2).repeat_interleave(G, 0)
+            vb = torch.stack([h[1] for h in hist[b]]).double().permute(1, 0, 2).repeat_interleave(G, 0)
+            qb = y[:, :Hq].double().permute(1, 0, 2)
+            s_ = qb @ kb.transpose(1, 2) / math.sqrt(D)
+            size = (qb.abs() @ kb.abs().transpose(1, 2) / math.sqrt(D)).amax(-1, keepdim=True)
+            see = torch.arange(p + n, device="cuda")[None] <= pos[:, None]
+            pr = torch.softmax(s_.masked_fill(~see, -math.inf), -1)
+            ref, A = pr @ vb, pr @ vb.abs()
+            # on top of the attention's own rounding, a q or k rounded the other way (rope in 32 bits against
+            # 64, ties aside) moves a score by at most e of its size
+            d = e * size + D * 2.0 ** -24 * size + 2.0 ** -20
+            tol = 1.01 * (e / 2 * ref.abs() + (e / 2 + 2 * d) * A)
+            got = out[at - n:at].double().permute(1, 0, 2)
+            assert ((got - ref).abs() <= tol).all(), (b, p, n)
+        assert (out[at:] == 9).all()
+    held = sum(n_blocks.tolist())
+    assert held + n_free.item() == num_pages
+    used = [i for b in range(B) for i in table[b].tolist() if i >= 0] + free[:n_free.item()].tolist()
+    assert sorted(used) == list(range(num_pages))
+    _no_device_error(ops)
+
+
+def test_serving_steps(ops):
+    _serve(ops, graph=False)
+
+
+def test_serving_steps_from_a_graph(ops):
+    """The same steps replayed from one captured graph: lengths, pages and splits are
+    all found on the device."""
+    _serve(ops, graph=True)
+
+
+def test_two_graphs_at_once(ops):
+    """Graphs captured one after the other share no workspace: replayed on two streams
+    at the same time, both are right."""
+    a, b = Paged([(9000, 1)], 28, 4, 128, 16, BF, seed=1), Paged([(7000, 2), (50, 3)], 28, 4, 128, 64, BF, seed=2)
+    want = [a.call(ops), b.call(ops)]
+    graphs, outs = [], []
+    for x in (a, b):
+        g = torch.cuda.CUDAGraph()
+        out = torch.zeros_like(x.q)
+        with torch.cuda.graph(g):
+            x.call(ops, out=out)
+        graphs.append(g)
+        outs.append(out)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(10):
+        for o in outs:
+            o.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, (s1, s2)):
+            with torch.cuda.stream(s):
+                for _ in range(4):
+                    g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    _no_device_error(ops)
