@@ -76,7 +76,7 @@ constexpr int PA_POLY = 4;  // every 4th pair of exponentials on the FMA pipe
 
 // What a CTA leaves for the merge about the item that its share ends inside.
 struct PagedSplit {
-  int last_cta;  // the item's last piece; < 0: nothing to merge
+  int first_cta, last_cta;  // where the item's pieces are; last < 0: nothing to merge
   int token0;    // first token row of the item
   int tokens;
   int kvh;
@@ -1213,7 +1213,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           walk.skip = off;
         }
       }
-      PagedSplit split = {-1, 0, 0, 0};
+      PagedSplit split = {0, -1, 0, 0, 0};
       bool more = true;
       for (uint32_t n = 0; more; ++n) {
         more = walk.next(p);
@@ -1230,9 +1230,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           mbar_arrive(&sh.bar_piece[i]);
         }
         __syncwarp();
-        if (more && walk.j0 == 0 && walk.j1 < walk.nb) {
+        if (more && walk.j1 < walk.nb) {
           // the share ends inside this item: a block lies with the CTA whose share holds its cost
-            const int start = x0 + share - walk.cut;
+          const int start = x0 + share - walk.cut;
+          split.first_cta = (start + ((PA_OVER * walk.w) >> p.unit_log2)) / share;
           split.last_cta = (start + (((walk.nb - 1 + PA_OVER) * walk.w) >> p.unit_log2)) / share;
           split.token0 = walk.q0 + walk.t0;
           split.tokens = walk.nt;
@@ -1251,8 +1252,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   }
 }
 
-// Joins the pieces of the items that cuts divide: blocks x look at the item
-// that CTA x's share ends inside.  out = sum_c w_c o_c / sum_c w_c l_c with w_c =
+// Joins the pieces of the items that cuts divide: blocks x work at the item that
+// CTA x's share ends inside, so an item of many pieces has many blocks.  out = sum_c w_c o_c / sum_c w_c l_c with w_c =
 // exp2(m_c - max m), in a fixed order of the pieces.  Latency is what counts (a
 // few loads per row, mostly from L2): the grid is one wave, since each wave of
 // blocks costs a memory round trip even where there is nothing to join, and the
@@ -1294,10 +1295,11 @@ __global__ void __launch_bounds__(PM_THREADS, 2) paged_merge_kernel(const PagedA
   constexpr int PER = D / 32;  // columns per lane
   const int cta = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedSplit sp = p.splits[cta];
-  if (sp.last_cta <= cta) return;
-  const int n = sp.last_cta - cta + 1;
-  // piece i is CTA cta + i's: its continued item (slot 0), or for the first the item begun there (slot 1)
-  auto slot = [&](int i) { return (static_cast<size_t>(2 * (cta + i)) + (i == 0 ? 1 : 0)) * 256; };
+  if (sp.last_cta <= cta || sp.first_cta > cta || sp.first_cta < 0) return;
+  const int n = sp.last_cta - sp.first_cta + 1;
+  const int block = (cta - sp.first_cta) * gridDim.y + blockIdx.y, blocks = (n - 1) * gridDim.y;  // of this item
+  // piece i is CTA first + i's: its continued item (slot 0), or for the first the item begun there (slot 1)
+  auto slot = [&](int i) { return (static_cast<size_t>(2 * (sp.first_cta + i)) + (i == 0 ? 1 : 0)) * 256; };
   auto load = [&](size_t row, bool there, float2& ml, float* o) {
     ml = make_float2(-INFINITY, 0.f);
 #pragma unroll
@@ -1332,7 +1334,7 @@ __global__ void __launch_bounds__(PM_THREADS, 2) paged_merge_kernel(const PagedA
   };
   if (n <= 8) {
     constexpr int ROWS = 2, WARPS = PM_THREADS / 32;
-    for (int r0 = (blockIdx.y * WARPS + warp) * ROWS; r0 < end; r0 += gridDim.y * WARPS * ROWS) {
+    for (int r0 = (block * WARPS + warp) * ROWS; r0 < end; r0 += blocks * WARPS * ROWS) {
       bool there[ROWS];
       PagedSum<D> sum[ROWS];
 #pragma unroll
@@ -1358,7 +1360,7 @@ __global__ void __launch_bounds__(PM_THREADS, 2) paged_merge_kernel(const PagedA
   __shared__ float s_o[ROWS][8][D];
   __shared__ float2 s_ml[ROWS][8];
   const int q = warp >> 3, part = warp & 7;
-  for (int r0 = blockIdx.y * ROWS; r0 < end; r0 += gridDim.y * ROWS) {
+  for (int r0 = block * ROWS; r0 < end; r0 += blocks * ROWS) {
     const int r = r0 + q;
     const bool there = row_there(r);
     if (!__syncthreads_or(there ? 1 : 0)) continue;  // (and the last rows' values have been read)
