@@ -57,7 +57,7 @@ constexpr int PA_BN = 128;       // keys per block
 constexpr float PA_RESCALE = 8.0f;  // log2 units
 // Cost of a block in a single and in a pair; an item costs PA_OVER blocks more
 // (its queries, first keys and output).
-constexpr int PA_W1 = 2, PA_W2 = 3, PA_OVER = 2;
+constexpr int PA_W1 = 3, PA_W2 = 5, PA_OVER = 3;
 constexpr int PA_WHOLE = 4;  // an item of at most this many blocks is not divided: it goes where it begins
 
 // Shared memory: two query slots and a ring of K/V blocks.  A slot holds a
