@@ -306,8 +306,8 @@ int std_collect_relevance(const void* q, const void* k_cache, const int32_t* vis
  * right after the take that it undoes restores tables and list exactly.
  * A request whose needed pages, with those of the requests before it, are more
  * than the list holds (after this call's returns) is refused: admitted[b] 0,
- * kv_lens[b] 0, its pages as before.  The others: admitted[b] 1, kv_lens[b] =
- * past + new.  cu_q [B + 1]: exclusive sums of new_lens, refused ones
+ * kv_lens[b] 0, its pages as before (the caller keeps its past length for the
+ * next step).  The others: admitted[b] 1, kv_lens[b] = past + new.  cu_q [B + 1]: exclusive sums of new_lens, refused ones
  * included.  slots, positions [max_tokens]: where token i of the step (request
  * order) goes; -1 for tokens of refused requests and past the last token.
  * max_tokens 0: neither is written (they may be NULL).
@@ -346,8 +346,9 @@ int std_paged_rope_append(const void* qkv, int T, int Hq, int Hkv, int D, int is
  * 3), the request skipped or its keys cut; a page id outside the pool is
  * reported (error 2) and read as zeros.
  * Same inputs, same bits; a request's last bits may depend on the batch it is
- * in (std_verify_attn's do not).  The workspace
- * (std_paged_attn_workspace_bytes) is that of one call at a time. */
+ * in (std_verify_attn's do not).  out and lse overlap no input.  The workspace
+ * (std_paged_attn_workspace_bytes, 32-byte aligned) is that of one call at a
+ * time. */
 size_t std_paged_attn_workspace_bytes(int D);
 int std_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int32_t* block_table,
                    const int32_t* cu_q, const int32_t* kv_lens, int T, int B, int Hq, int Hkv, int D, int is_fp16,

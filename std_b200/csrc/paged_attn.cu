@@ -106,7 +106,6 @@ STD_DEV bool paged_request(const PagedAttnParams& p, int q0, int q1, int& kv, in
   kv = kv < 0 ? 0 : (kv > room ? room : kv);
   return fit;
 }
-STD_DEV int paged_kv(const PagedAttnParams& p, int b) { return min(max(__ldg(p.kv_lens + b), 0), p.width << p.page_log2); }
 // Inclusive sums over the warp's lanes.
 STD_DEV int warp_scan(int v, int lane) {
 #pragma unroll
@@ -283,15 +282,6 @@ STD_DEV void tmem_ld_cols(uint32_t taddr, uint32_t* r) {
   } else {
 #pragma unroll
     for (int c = 0; c < N / 32; ++c) tmem_ld32(taddr + 32 * c, r + 32 * c);
-  }
-}
-template <int N>
-STD_DEV void tmem_st_cols(uint32_t taddr, const uint32_t* r) {
-  if constexpr (N == 16) {
-    tmem_st16(taddr, r);
-  } else {
-#pragma unroll
-    for (int c = 0; c < N / 32; ++c) tmem_st32(taddr + 32 * c, r + 32 * c);
   }
 }
 // One thread of a converged warp, the same one each time.  Behind this predicate
@@ -489,8 +479,7 @@ STD_DEV int warp_reduce_rows(float* v, int lane, Op op) {
 template <typename T, int D, int N, int ST>
 STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, PagedShared<ST>& sh, uint8_t* sQ,
                              uint8_t* sV, uint32_t tS, uint32_t tO, int s, uint64_t* bar_q_empty, uint32_t& ntail,
-                             uint32_t& ns, uint32_t& no, uint32_t& nj,
-                             uint32_t& ng) {
+                             uint32_t& ns, uint32_t& no, uint32_t& nj, uint32_t& ng) {
   const int tid = threadIdx.x, lane = tid & 31, w = (tid >> 5) & 3, key = tid & 127;
   const int rows = piece.tokens * p.G, steps = (piece.nblk - s + 1) >> 1;
   const float sc = p.scale_log2;
@@ -662,9 +651,9 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
 
 template <typename T, int D>
 __global__ void __launch_bounds__(PA_THREADS, 1)
-    paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ,
-                      const __grid_constant__ CUtensorMap tmQfew, const __grid_constant__ CUtensorMap tmK,
-                      const __grid_constant__ CUtensorMap tmV, const PagedAttnParams p) {
+    paged_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmQfew,
+                      const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                      const PagedAttnParams p) {
   typedef PagedTile<D> Tile;
   constexpr int ST = Tile::stages;
   constexpr int HALVES = D / 64;
@@ -779,7 +768,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(half == 0 ? &sh.bar_p[s] : &sh.bar_p2[s]);
       }
-      if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_s[s][0], ns++ & 1));  // (the commit after the last P V)
+      // (the commit in place of the S after the last)
+      if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_s[s][0], ns++ & 1));
       // ---- the item's result ----
       if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_o[s], no++ & 1));
       if (!ok) break;
@@ -815,31 +805,31 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const size_t orow = static_cast<size_t>(token) * p.Hq + head;
         const size_t slot = static_cast<size_t>(whole ? 0 : piece.slot) * 256 + tile * 128 + r;
 #pragma unroll 1
-        for (int piece = 0; piece < D / 32; ++piece) {
+        for (int c = 0; c < D; c += 32) {
           uint32_t oa[32];
           float v[32];
-          tmem_ld32(tO + piece * 32, oa);
+          tmem_ld32(tO + c, oa);
           tmem_wait_ld();
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = seen_a ? __uint_as_float(oa[j]) * wa : 0.f;
           if (join) {
-            tmem_ld32(tO + 128 + piece * 32, oa);
+            tmem_ld32(tO + 128 + c, oa);
             tmem_wait_ld();
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] += seen_b ? __uint_as_float(oa[j]) * wb : 0.f;
           }
           if (valid_row) {
             if (whole) {
-              T* dst = static_cast<T*>(p.out) + orow * D + piece * 32;
+              T* dst = static_cast<T*>(p.out) + orow * D + c;
               uint32_t pk[16];
 #pragma unroll
               for (int j = 0; j < 16; ++j) pk[j] = pack_pair<T>(v[2 * j] * inv, v[2 * j + 1] * inv);
               st_global_32b(dst, pk, p.out_32b);
               st_global_32b(dst + 16, pk + 8, p.out_32b);
             } else {
-              float* dst = p.ws_o + slot * D + piece * 32;
+              float* dst = p.ws_o + slot * D + c;
 #pragma unroll
-              for (int c = 0; c < 4; ++c) st_global_32b(dst + 8 * c, reinterpret_cast<const uint32_t*>(v) + 8 * c, true);
+              for (int j = 0; j < 32; j += 8) st_global_32b(dst + j, reinterpret_cast<const uint32_t*>(v) + j, true);
             }
           }
         }
@@ -886,9 +876,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           return lane < per_block && j < piece.j0 + nblk && key < limit ? __ldg(row + (key >> p.page_log2)) : 0;
         };  // (not looked at before it is used: the load is on its way meanwhile)
         int next_id = page_of(piece.j0);
-        // queries; a whole tile may take its slot's last half only when the few-row
-        // piece before it is done there
-        if (was_few && !few) ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_q_empty[(nq - 1) & 1], ((nq - 1) >> 1) & 1));
+        // queries; between whole tiles and few rows, which use a slot's last half
+        // differently (the latter both slots', whichever holds the queries), the last
+        // tile has to be done with its slot, not only the one before it
+        if (nq > 0 && was_few != few)
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_q_empty[(nq - 1) & 1], ((nq - 1) >> 1) & 1));
         was_few = few;
         for (int s = 0; ok && s < (pair ? 2 : 1); ++s, ++nq) {
           const int st = nq & 1;
@@ -1295,7 +1287,8 @@ __global__ void __launch_bounds__(PM_THREADS, 2) paged_merge_kernel(const PagedA
   constexpr int PER = D / 32;  // columns per lane
   const int cta = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedSplit sp = p.splits[cta];
-  if (sp.last_cta <= cta || sp.first_cta > cta || sp.first_cta < 0) return;
+  // (the rest only if cu_q overlaps itself: the sums it gives may pass 32 bits)
+  if (sp.last_cta <= cta || sp.first_cta > cta || sp.first_cta < 0 || sp.last_cta >= PA_CTAS) return;
   const int n = sp.last_cta - sp.first_cta + 1;
   const int block = (cta - sp.first_cta) * gridDim.y + blockIdx.y, blocks = (n - 1) * gridDim.y;  // of this item
   // piece i is CTA first + i's: its continued item (slot 0), or for the first the item begun there (slot 1)
@@ -1428,6 +1421,13 @@ static int paged_attn_launch(const CUtensorMap& tq, const CUtensorMap& tqf, cons
                              const stdb::PagedAttnParams& p, cudaStream_t s) {
   static SmemGrant grant;
   if (ensure_smem(stdb::paged_attn_kernel<T, D>, grant, stdb::PagedTile<D>::smem) != 0) return 3;
+  // The warpgroups' register shares must not add up to more than the launch has:
+  // setmaxnreg would wait for ever.
+  static const int regs = [] {
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, stdb::paged_attn_kernel<T, D>) == cudaSuccess ? a.numRegs : 0;
+  }();
+  if (regs * stdb::PA_THREADS < 256 * stdb::PA_REGS_SOFTMAX + 128 * stdb::PA_REGS_OTHER) return 3;
   if (launch_pdl(stdb::paged_attn_kernel<T, D>, dim3(stdb::PA_CTAS), dim3(stdb::PA_THREADS), stdb::PagedTile<D>::smem,
                  s, tq, tqf, tk, tv, p) != cudaSuccess)
     return 4;
