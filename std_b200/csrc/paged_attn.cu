@@ -43,6 +43,21 @@
 // of 128 rows has constant strides.  Only pages with a visible key are read.
 // Rows past the last visible key may hold anything: their scores are replaced,
 // not added to, and their V rows are cleared before the product.
+//
+// What bounds it, and what was measured (B200, replayed from a graph; bf16, 28
+// query heads on 4 key heads, D 128 unless said).  Long prompts: a 2048-token
+// chunk over 31K keys 815 us = 1150 TFLOP/s (0.84 of what cuBLAS sustains under
+// the power cap; ncu: tensor pipe 58 % by its own MMAs' time, 71 % counting
+// operand reads; clock 1.65 GHz), an 8192-token prompt 450-530 us as the clock
+// allows.  S in halves costs 1.5 x the shared-memory reads of N=128 but keeps a
+// half of S ready while the other is multiplied: 866 us with one S of 128 columns
+// a step from one issuing thread, 815 with halves and a thread per stream.
+// Decoding: HBM; 64 requests of 100 to 8000 keys 85 us = 5.7 TB/s (0.88 of the
+// measured copy), one request of 131K keys 50 us = 5.4 TB/s, 8 verify blocks of
+// 10 tokens over 33K keys 99 us = 5.4 TB/s; untransposed, the first two took 118
+// and 67 us, bound by one warp's softmax of 128 columns for 7 live rows.  Short
+// contexts: latency, 7.5 us for one token and 200 keys, half of it finding the
+// share (2 us) and the first page, key and score (2 us).
 #include "common.cuh"
 
 #include <type_traits>
@@ -55,10 +70,14 @@ constexpr int PA_THREADS = 384;  // 2 softmax warpgroups; TMA, two MMA and a sch
 constexpr int PA_REGS_SOFTMAX = 208, PA_REGS_OTHER = 88;
 constexpr int PA_BN = 128;       // keys per block
 constexpr float PA_RESCALE = 8.0f;  // log2 units
-// Cost of a block in a single and in a pair; an item costs PA_OVER blocks more
-// (its queries, first keys and output).
+// Cost of a block in a single and in a pair (measured: 2000 to 2400 cycles and
+// 3700); an item costs PA_OVER blocks more (its queries, first keys and output).
 constexpr int PA_W1 = 3, PA_W2 = 5, PA_OVER = 3;
-constexpr int PA_WHOLE = 4;  // an item of at most this many blocks is not divided: it goes where it begins
+// An item of at most this many blocks is not divided but goes where it begins: a cut
+// would cost a partial and the merge (2 us) to save at most two blocks (2 us), and
+// calls whose tables allow no longer item need no merge launch (9.6 -> 7.7 us for
+// one token and 200 keys).
+constexpr int PA_WHOLE = 4;
 
 // Shared memory: two query slots and a ring of K/V blocks.  A slot holds a
 // 128-row Q tile (halves of 64 columns, 16 KB apart), or, for few rows, a 32-row
@@ -71,8 +90,12 @@ struct PagedTile {
   static constexpr int stages = D == 128 ? 5 : 8;
   static constexpr uint32_t smem = 2 * PA_SLOT + stages * kv_bytes + 1024;
 };
-constexpr int PA_FEW = 32;  // most rows of an item that is computed transposed
-constexpr int PA_POLY = 4;  // every 4th pair of exponentials on the FMA pipe
+// Most rows of an item that is computed transposed.  Up to 64 it would still pay by
+// itself, but the registers of that variant (64 scores and 64 sums a thread) made
+// the compiler spill in the whole-tile softmax beside it: 8 verify blocks over 33K
+// keys 105 -> 99 us, an 8192-token prompt 505 -> 455 us without it.
+constexpr int PA_FEW = 32;
+constexpr int PA_POLY = 4;  // every 4th pair of exponentials on the FMA pipe (chunk: none 846 us, a half 875, a quarter 820)
 
 // What a CTA leaves for the merge about the item that its share ends inside.
 struct PagedSplit {
@@ -428,7 +451,7 @@ STD_DEV bool paged_softmax_half(uint32_t tS, uint32_t tO, float sc, int nvis, fl
   for (int j = 0; j < N / 2; ++j) {
     const uint64_t y = f2_fma(f2_make(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), sc2, nm2);
     float2 e;
-    if (PA_POLY > 0 && j % PA_POLY == PA_POLY - 1) {
+    if (j % PA_POLY == PA_POLY - 1) {
       e = ex2_fma2(y);
     } else {
       e = f2_split(y);

@@ -27,7 +27,8 @@ namespace stdb {
 // page moves, all latency.  Prefix sums live in shared memory, and every later
 // phase (returns, takes, tokens) is flat over its own items, each finding its
 // request by bisection: the time does not depend on how the pages and tokens
-// are spread over the requests.
+// are spread over the requests.  Measured (from a graph): 3.1 us for 8 requests of
+// 10 new tokens, 5.5 us for 256 requests with 8192 new tokens.
 struct PagedUpdateParams {
   const int32_t* past;
   const int32_t* fresh;
@@ -120,13 +121,15 @@ __global__ void __launch_bounds__(1024) paged_update_kernel(const PagedUpdatePar
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-      long long before = run[i];
-      for (int w = 0; w < nw; ++w) {
-        const long long part = s_part[i][w];
-        if (w < warp) before += part;
-        run[i] += part;
+      long long part = lane < nw ? s_part[i][lane] : 0;  // the warps' sums, scanned by every warp
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, part, o);
+        if (lane >= o) part += u;
       }
-      inc[i] += before;
+      const long long before = __shfl_sync(0xffffffffu, part, warp > 0 ? warp - 1 : 0);
+      inc[i] += run[i] + (warp > 0 ? before : 0);
+      run[i] += __shfl_sync(0xffffffffu, part, 31);
     }
     if (b < p.B) {
       // sums beyond int32 only arise from lengths that no table holds; they are
@@ -218,7 +221,9 @@ __global__ void __launch_bounds__(256) paged_tokens_kernel(const PagedUpdatePara
 // y_lo = lo cos - hi sin, y_hi = hi cos + lo sin over the two halves of each q
 // and k head, in fp32 and rounded once (the contiguous rope_append rounds every
 // product to bf16, as the reference's bf16 arithmetic does); v is copied.  A
-// thread handles 8 + 8 elements (16-byte loads and stores), a block one token.
+// thread handles 8 + 8 elements (16-byte loads and stores), a block one token:
+// HBM, 8192 tokens of 28 + 8 heads 28.7 us = 5.3 TB/s read and written (0.81 of the
+// measured copy); 80 tokens 1.8 us.
 struct PagedAppendParams {
   const void* qkv;  // [T, (Hq + 2 Hkv) * D]
   const int32_t* positions;
@@ -350,7 +355,10 @@ extern "C" int std_paged_update(const int32_t* past_lens, const int32_t* new_len
   p.slots = slots;
   p.positions = positions;
   p.admitted = admitted;
-  p.tokens_here = max_tokens <= 4096 ? 1 : 0;
+  // Few tokens' slots are written by the one block, many by a second kernel of many
+  // blocks (8 requests: 256 tokens 3.2 us against 4.3, 1024 4.3 against 4.5, 4096
+  // 6.4 against 4.4; 256 requests: 1024 tokens 4.7 against 5.4, 4096 7.6 against 5.4).
+  p.tokens_here = max_tokens <= 1024 ? 1 : 0;
   const size_t smem = (4 * static_cast<size_t>(B) + 1) * 4;
   static SmemGrant grant;
   if (ensure_smem(stdb::paged_update_kernel, grant, smem) != 0) return 3;
