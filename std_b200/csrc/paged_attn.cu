@@ -66,8 +66,8 @@ namespace stdb {
 
 constexpr int PA_CTAS = 148;     // one CTA per SM
 constexpr int PA_THREADS = 384;  // 2 softmax warpgroups; TMA, two MMA and a scheduler warp
-// Registers after the split: 2 * 128 * 208 + 128 * 88 = 384 * 168, the launch's total.
-constexpr int PA_REGS_SOFTMAX = 208, PA_REGS_OTHER = 88;
+// Registers after the split: 2 * 128 * 192 + 128 * 120 = 384 * 168, the launch's total.
+constexpr int PA_REGS_SOFTMAX = 192, PA_REGS_OTHER = 120;
 constexpr int PA_BN = 128;       // keys per block
 constexpr float PA_RESCALE = 8.0f;  // log2 units
 // Cost of a block in a single and in a pair (measured: 2000 to 2400 cycles and
@@ -95,7 +95,9 @@ struct PagedTile {
 // the compiler spill in the whole-tile softmax beside it: 8 verify blocks over 33K
 // keys 105 -> 99 us, an 8192-token prompt 505 -> 455 us without it.
 constexpr int PA_FEW = 32;
-constexpr int PA_POLY = 4;  // every 4th pair of exponentials on the FMA pipe (chunk: none 846 us, a half 875, a quarter 820)
+// Every 3rd pair of exponentials goes to the FMA pipe (the 2048-token chunk in a
+// long run: none 972 us, every 8th 950, 4th 947, 3rd 942; every 2nd is slower again).
+constexpr int PA_POLY = 3;
 
 // What a CTA leaves for the merge about the item that its share ends inside.
 struct PagedSplit {
