@@ -66,8 +66,6 @@ namespace stdb {
 
 constexpr int PA_CTAS = 148;     // one CTA per SM
 constexpr int PA_THREADS = 384;  // 2 softmax warpgroups; TMA, two MMA and a scheduler warp
-// Registers after the split: 2 * 128 * 192 + 128 * 120 = 384 * 168, the launch's total.
-constexpr int PA_REGS_SOFTMAX = 192, PA_REGS_OTHER = 120;
 constexpr int PA_BN = 128;       // keys per block
 constexpr float PA_RESCALE = 8.0f;  // log2 units
 // Cost of a block in a single and in a pair (measured: 2000 to 2400 cycles and
@@ -729,7 +727,6 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
   };
 
   if (warp < 8) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PA_REGS_SOFTMAX));
     // ---------------- softmax warpgroups: thread = row ----------------
     const int s = warp >> 2, r = tid & 127;
     const uint32_t trow = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -880,7 +877,6 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_OTHER));
     if (warp == 8) {
       // ---------------- TMA producer: the whole warp, a page per lane ----------------
       const int box_log2 = min(p.page_log2, 7), box = 1 << box_log2;  // rows per copy
@@ -1446,13 +1442,6 @@ static int paged_attn_launch(const CUtensorMap& tq, const CUtensorMap& tqf, cons
                              const stdb::PagedAttnParams& p, cudaStream_t s) {
   static SmemGrant grant;
   if (ensure_smem(stdb::paged_attn_kernel<T, D>, grant, stdb::PagedTile<D>::smem) != 0) return 3;
-  // The warpgroups' register shares must not add up to more than the launch has:
-  // setmaxnreg would wait for ever.
-  static const int regs = [] {
-    cudaFuncAttributes a;
-    return cudaFuncGetAttributes(&a, stdb::paged_attn_kernel<T, D>) == cudaSuccess ? a.numRegs : 0;
-  }();
-  if (regs * stdb::PA_THREADS < 256 * stdb::PA_REGS_SOFTMAX + 128 * stdb::PA_REGS_OTHER) return 3;
   if (launch_pdl(stdb::paged_attn_kernel<T, D>, dim3(stdb::PA_CTAS), dim3(stdb::PA_THREADS), stdb::PagedTile<D>::smem,
                  s, tq, tqf, tk, tv, p) != cudaSuccess)
     return 4;
