@@ -630,3 +630,87 @@ def test_two_graphs_at_once(ops):
         torch.cuda.synchronize()
         assert all(torch.equal(o, w) for o, w in zip(outs, want))
     _no_device_error(ops)
+
+
+# ------------------------------------------------------------------ extremes
+def test_attention_wide_tables(ops):
+    """Tables that allow requests of 2^31 keys: costs are counted in coarser units,
+    the shares stay a partition of the blocks."""
+    x = Paged([(3000, 1), (700, 40), (0, 300), (5000, 2), (90, 1), (1, 1), (2000, 9), (12, 130)], 28, 4, 128, 256, BF,
+              seed=6)
+    wide = torch.full((8, 8388600), -1, dtype=torch.int32, device="cuda")
+    wide[:, :x.table.shape[1]] = x.table
+    out = torch.empty_like(x.q)
+    lse = torch.empty(x.q.shape[:2], device="cuda")
+    ops.paged_attention(x.q, x.k, x.v, wide, x.cu, x.kv_lens, out=out, lse=lse)
+    x.check(out, lse)
+    _no_device_error(ops)
+
+
+@pytest.mark.parametrize("offset", [8, 16, 24])
+def test_attention_tensors_inside_others(ops, offset):
+    """Tensors that begin 16 bytes into an allocation (16-byte, not 32-byte aligned)."""
+    x = Paged([(300, 1), (70, 60), (2500, 9)], 28, 4, 128, 64, BF, seed=offset)
+    want = x.call(ops)
+
+    def inside(t):
+        room = torch.zeros(t.numel() + offset, dtype=t.dtype, device="cuda")
+        view = room[offset:].view(t.shape)
+        view.copy_(t)
+        return view
+
+    out = inside(torch.zeros_like(x.q))
+    got = ops.paged_attention(inside(x.q), inside(x.k), inside(x.v), inside(x.table), inside(x.cu), inside(x.kv_lens),
+                              out=out)
+    assert torch.equal(got, want)
+    with pytest.raises(RuntimeError, match="status 1"):
+        room = torch.zeros(x.q.numel() + 1, dtype=BF, device="cuda")
+        ops.paged_attention(x.q, x.k, x.v, x.table, x.cu, x.kv_lens, out=room[1:].view(x.q.shape))
+    _no_device_error(ops)
+
+
+def test_attention_most_requests_and_many_heads(ops):
+    rng = random.Random(8192)
+    x = Paged([(rng.randint(0, 40), rng.choice([0, 1, 1, 2])) for _ in range(8192)], 2, 1, 64, 16, FP, seed=3)
+    out = x.call(ops)
+    for b in (0, 1, 4095, 8190, 8191):  # (the 64-bit check of all would take minutes)
+        n = x.pairs[b][1]
+        one = Paged.__new__(Paged)
+        at = x.cu[b].item()
+        one.__dict__.update(x.__dict__, pairs=[x.pairs[b]], kv=[x.kv[b]], keys=[x.keys[b]], q=x.q[at:at + n])
+        one.check(out[at:at + n], None)
+    assert torch.isfinite(out).all()
+    x = Paged([(100, 3), (9, 1), (700, 140)], 300, 300, 64, 32, BF, seed=4)
+    x.check(x.call(ops), None)
+    _no_device_error(ops)
+
+
+def test_long_prompt_whole_and_in_chunks(ops):
+    """A 40,000-token prompt at once and in odd chunks: the same rows within their rounding."""
+    Hq, Hkv, D, page, n = 14, 2, 128, 128, 40000
+    g = torch.Generator(device="cuda").manual_seed(1)
+    blocks = -(-n // page)
+    q = torch.randn(n, Hq, D, generator=g, device="cuda").to(BF)
+    k = torch.randn(blocks, Hkv, page, D, generator=g, device="cuda").to(BF)
+    v = torch.randn(blocks, Hkv, page, D, generator=g, device="cuda").to(BF)
+    table = torch.randperm(blocks, generator=g, device="cuda").int().view(1, -1)
+    whole = ops.paged_attention(q, k, v, table, _i32([0, n]), _i32([n]))
+    at = 0
+    for size in (1, 17, 5000, 13001, 36, 21944, 1):
+        part = ops.paged_attention(q[at:at + size], k, v, table, _i32([0, size]), _i32([at + size]))
+        # each is off from the exact row by at most e/2 (|o| + A), A <= max |v| here taken as 6
+        off = (part.double() - whole[at:at + size].double()).abs()
+        assert (off <= 2 * 2.0 ** -8 * (whole[at:at + size].double().abs() + 6)).all()
+        assert off.mean() < 1e-3
+        at += size
+    assert at == n
+    # rows near the end against 64 bits
+    kk = k[table[0].long()].permute(1, 0, 2, 3).reshape(Hkv, -1, D)[:, :n].double()
+    vv = v[table[0].long()].permute(1, 0, 2, 3).reshape(Hkv, -1, D)[:, :n].double()
+    for row in (n - 1, n - 129, 20000):
+        s = torch.einsum("hd,hld->hl", q[row].double(), kk[:, :row + 1].repeat_interleave(7, 0)) / math.sqrt(D)
+        p = torch.softmax(s, -1)
+        ref = torch.einsum("hl,hld->hd", p, vv[:, :row + 1].repeat_interleave(7, 0))
+        A = torch.einsum("hl,hld->hd", p, vv[:, :row + 1].abs().repeat_interleave(7, 0))
+        assert ((whole[row].double() - ref).abs() <= 1.02 * 2.0 ** -8 * (ref.abs() + A)).all()
+    _no_device_error(ops)
