@@ -132,8 +132,8 @@ __global__ void __launch_bounds__(1024) paged_update_kernel(const PagedUpdatePar
       run[i] += __shfl_sync(0xffffffffu, part, 31);
     }
     if (b < p.B) {
-      // sums beyond int32 only arise from lengths that no table holds; they are
-      // reported below and cut here so that every index stays in range
+      // sums beyond int32 are reported below and cut here so that every index stays
+      // in range; a request's own tokens are read from `fresh`, not from these
       s_cu[b] = static_cast<int>(min(inc[0] - v[0], 0x7fffffffll));
       s_take[b] = static_cast<int>(inc[1] - v[1]);
       s_back[b] = static_cast<int>(inc[2] - v[2]);
@@ -144,8 +144,9 @@ __global__ void __launch_bounds__(1024) paged_update_kernel(const PagedUpdatePar
   const int back = static_cast<int>(run[2]);
   if (tid == 0) {
     s_cu[p.B] = static_cast<int>(min(run[0], 0x7fffffffll));
-    // more tokens than the outputs hold, or more pages returned than exist
-    if (run[0] > p.max_tokens) std_set_error(STD_DEVERR_LENGTH);
+    // more tokens than the outputs hold (cu_q, or slots and positions if there are
+    // any), or more pages returned than exist
+    if (run[0] > (p.max_tokens > 0 ? p.max_tokens : 0x7fffffffll)) std_set_error(STD_DEVERR_LENGTH);
     if (static_cast<long long>(n_free) + back > p.num_pages) std_set_error(STD_DEVERR_BOUNDS);
   }
   // returns: page r of the whole step, ids cleared from the table
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(1024) paged_update_kernel(const PagedUpdatePar
   for (int b = tid; b < p.B; b += nt) {
     const int past = s_past[b], needs = (b + 1 < p.B ? s_take[b + 1] : need) - s_take[b];
     const bool ok = past >= 0 && (needs == 0 || s_take[b] + needs <= taken);
-    const long long len = static_cast<long long>(past) + (s_cu[b + 1] - s_cu[b]);
+    const long long len = static_cast<long long>(past) + p.fresh[b];
     p.cu_q[b] = s_cu[b];
     p.kv_lens[b] = ok ? static_cast<int>(len) : 0;
     p.admitted[b] = ok ? 1 : 0;
@@ -212,8 +213,7 @@ __global__ void __launch_bounds__(256) paged_tokens_kernel(const PagedUpdatePara
     p.slots[t] = -1;
     p.positions[t] = -1;
   } else {
-    const int n = p.cu_q[b + 1] - p.cu_q[b];
-    paged_token(p, p.table + static_cast<size_t>(b) * p.width, p.kv_lens[b] - n + (t - p.cu_q[b]), t);
+    paged_token(p, p.table + static_cast<size_t>(b) * p.width, p.kv_lens[b] - p.fresh[b] + (t - p.cu_q[b]), t);
   }
 }
 

@@ -714,3 +714,56 @@ def test_long_prompt_whole_and_in_chunks(ops):
         A = torch.einsum("hl,hld->hd", p, vv[:, :row + 1].abs().repeat_interleave(7, 0))
         assert ((whole[row].double() - ref).abs() <= 1.02 * 2.0 ** -8 * (ref.abs() + A)).all()
     _no_device_error(ops)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_non_finite_keys_reach_those_who_see_them(ops, bad, D):
+    """A NaN or infinite score makes the rows that see it NaN, whatever its column and
+    its request's form (few rows, one tile, a pair, divided over CTAs), and no other."""
+    x = Paged([(300, 1), (290, 4), (290, 15), (200, 100), (6000, 2)], 28, 4, D, 64, BF, seed=12)
+    x.q[..., 0] = x.q[..., 0].abs() + 0.1  # (the score is +inf, not -inf)
+    lse0, lse = torch.empty(x.q.shape[:2], device="cuda"), torch.empty(x.q.shape[:2], device="cuda")
+    good = x.call(ops, lse=lse0)
+    for key in (0, 1, 2, 3, 4, 5, 62, 67, 130, 131, 132, 259, 290, 291, 295, 299, 300):
+        k = x.k.clone()
+        want, wlse, at = good.clone(), lse0.clone(), 0
+        for b, (past, n) in enumerate(x.pairs):
+            if key < past + n:
+                k[x.table[b, key // 64].item(), 1, key % 64, 0] = bad
+                first = max(0, key - past)  # the first of its tokens that sees it
+                want[at + first:at + n, 7:14] = math.nan
+                wlse[at + first:at + n, 7:14] = math.nan
+            at += n
+        out = ops.paged_attention(x.q, k, x.v, x.table, x.cu, x.kv_lens, lse=lse)
+        assert torch.equal(out.isnan(), want.isnan()) and torch.equal(lse.isnan(), wlse.isnan()), key
+        assert torch.equal(out.nan_to_num(7.0), want.nan_to_num(7.0)), key
+        assert torch.equal(lse.nan_to_num(7.0), wlse.nan_to_num(7.0)), key
+    _no_device_error(ops)
+
+
+@pytest.mark.parametrize("max_tokens", [0, 16, 2000])
+def test_update_after_a_length_of_2_31(ops, max_tokens):
+    """Requests behind refused ones whose lengths add up beyond 32 bits are served in
+    full: their pages are those that were taken."""
+    big = 2 ** 31 - 1
+    table, held = torch.full((4, 8), -1, dtype=torch.int32, device="cuda"), _i32([0, 0, 0, 0])
+    free, n_free = torch.arange(8, dtype=torch.int32, device="cuda"), _i32([8])
+    cu, kv, slots, pos, ok = ops.paged_update(_i32([0, 0, 0, 16]), _i32([big, 5, big, 33]), table, held, free, n_free,
+                                              16, max_tokens)
+    assert ops.device_error() == 3
+    assert ok.tolist() == [0, 1, 0, 1] and kv.tolist() == [0, 5, 0, 49]
+    assert held.tolist() == [0, 1, 0, 4] and n_free.tolist() == [3]
+    assert sorted(table[table >= 0].tolist()) == [3, 4, 5, 6, 7]
+    assert cu.tolist() == [0, big, big, big, big] and (slots == -1).all() and (pos == -1).all()
+    _no_device_error(ops)
+
+
+def test_update_tables_alone(ops):
+    """max_tokens 0: the tables without slots, for any number of new tokens."""
+    table, held = torch.full((2, 8), -1, dtype=torch.int32, device="cuda"), _i32([0, 0])
+    free, n_free = torch.arange(8, dtype=torch.int32, device="cuda"), _i32([8])
+    cu, kv, slots, pos, ok = ops.paged_update(_i32([0, 0]), _i32([20, 3]), table, held, free, n_free, 16, 0)
+    assert cu.tolist() == [0, 20, 23] and kv.tolist() == [20, 3] and ok.tolist() == [1, 1]
+    assert table[:, :2].tolist() == [[7, 6], [5, -1]] and slots.numel() == pos.numel() == 0
+    _no_device_error(ops)
