@@ -357,16 +357,23 @@ STD_DEV float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// (NaN if one of them is)
+STD_DEV float max2_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 // 2^y for two y <= 127 on the FMA and integer pipes, to spare the SFU (16
 // results a cycle and SM): y = n + f with n whole and |f| <= 1/2, 2^f = 1 + f q(f)
 // with q the degree-4 polynomial that interpolates (2^f - 1) / f at the Chebyshev
 // nodes of [-1/2, 1/2] (off by at most 2.1e-7, 2.6e-7 as rounded here), n added
 // to the exponent.  At and below -127 (masked: -inf) the sum is exactly 0, since
-// 2^0 is exactly 1 here; between that and -126 a number below 2^-126.
+// 2^0 is exactly 1 here; between that and -126 a number below 2^-126.  A NaN gives
+// FLT_MAX: n is added to the bits of a NaN.
 STD_DEV float2 ex2_fma2(uint64_t y2) {
   float2 y = f2_split(y2);
-  y.x = fmaxf(y.x, -127.f);
-  y.y = fmaxf(y.y, -127.f);
+  y.x = max2_nan(y.x, -127.f);
+  y.y = max2_nan(y.y, -127.f);
   const float MAGIC = 12582912.f;  // 1.5 * 2^23: adding it leaves round(y) in the low bits
   const uint64_t v = f2_make(y.x, y.y);
   const uint64_t t = f2_add(v, f2_make(MAGIC, MAGIC));
@@ -465,7 +472,10 @@ STD_DEV bool paged_softmax_half(uint32_t tS, uint32_t tO, float sc, int nvis, fl
   tmem_wait_st();
   tc_fence_before();
   const float2 l = f2_split(f2_add(l2[0], l2[1]));
+  // A NaN or infinite score makes its row NaN: it has left a NaN here or, through
+  // ex2_fma2, FLT_MAX or more; sums of numbers stay below 2^31 2^PA_RESCALE.
   l_run = l.x + l.y;
+  if (!(l_run < 1e30f)) l_run = NAN;
   return true;
 }
 
@@ -1466,6 +1476,8 @@ extern "C" int std_paged_attn(const void* q, const void* k_pages, const void* v_
       static_cast<long long>(num_pages) * page_size > 0x7fffffffll ||
       (static_cast<long long>(num_pages) + 1) * Hkv * (page_size / 8) > 0x7fffffffll || T > 0x7fffffff / 2)
     return 1;
+  // items, each of a cost of one or more, in a total of 32 bits (no memory holds more)
+  if ((static_cast<double>(T) / (2 * (128 / (Hq / Hkv))) + B) * Hkv > 5.0e8) return 1;
   if (T == 0) return 0;
   if (q == nullptr || k_pages == nullptr || v_pages == nullptr || block_table == nullptr || cu_q == nullptr ||
       kv_lens == nullptr || out == nullptr || q == out)

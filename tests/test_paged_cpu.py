@@ -27,6 +27,11 @@ def test_attention_refusals(bad):
     assert attn(**bad) == 1
 
 
+@pytest.mark.parametrize("bad", [dict(B=8192, Hkv=65535, Hq=65535), dict(T=1 << 30, Hkv=2000, Hq=256000)])
+def test_attention_refuses_more_items_than_32_bits_count(bad):
+    assert attn(pages=100, **bad) == 1
+
+
 def test_attention_workspace_and_nothing_to_do():
     need = _lib.query("std_paged_attn_workspace_bytes", 128)
     assert need > 0 and _lib.query("std_paged_attn_workspace_bytes", 96) == 0
