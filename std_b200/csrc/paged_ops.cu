@@ -221,9 +221,10 @@ __global__ void __launch_bounds__(256) paged_tokens_kernel(const PagedUpdatePara
 // y_lo = lo cos - hi sin, y_hi = hi cos + lo sin over the two halves of each q
 // and k head, in fp32 and rounded once (the contiguous rope_append rounds every
 // product to bf16, as the reference's bf16 arithmetic does); v is copied.  A
-// thread handles 8 + 8 elements (16-byte loads and stores), a block one token:
-// HBM, 8192 tokens of 28 + 8 heads 28.7 us = 5.3 TB/s read and written (0.81 of the
-// measured copy); 80 tokens 1.8 us.
+// thread handles 8 + 8 elements (16-byte loads and stores), a block one token.  The
+// row's loads go out before its position is there (28.6 -> 25.7 us).  HBM: 8192
+// tokens of 28 + 8 heads 25.7 us = 6.0 TB/s read and written (0.91 of the measured
+// copy); 80 tokens 1.6 us.
 struct PagedAppendParams {
   const void* qkv;  // [T, (Hq + 2 Hkv) * D]
   const int32_t* positions;
@@ -263,6 +264,13 @@ STD_DEV uint32_t pack_pair(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// A load that stays where it is written.
+STD_DEV uint4 ld_global_16b(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(512) paged_append_kernel(const PagedAppendParams p) {
   typedef typename PairOf<T>::type Pair;
@@ -271,16 +279,16 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const PagedAppendPara
   const int row = blockIdx.x;
   int pos = p.positions[row];
   const int slot = p.slots[row];
-  if (pos < 0) return;  // no token in this row
   const bool slot_ok = slot >= 0 && slot < p.total_slots;
-  if (threadIdx.x == 0 && (slot >= p.total_slots || pos >= p.max_pos)) std_set_error(STD_DEVERR_BOUNDS);
-  if (pos >= p.max_pos) pos = p.max_pos - 1;
   const int heads = p.Hq + 2 * p.Hkv, half = p.D / 2, per_head = half / 8;
   const T* src = static_cast<const T*>(p.qkv) + static_cast<size_t>(row) * heads * p.D;
   for (int i = threadIdx.x; i < heads * per_head; i += blockDim.x) {
     const int h = i / per_head, c = (i % per_head) * 8;
-    const uint4 lo = *reinterpret_cast<const uint4*>(src + h * p.D + c);
-    const uint4 hi = *reinterpret_cast<const uint4*>(src + h * p.D + half + c);
+    // (on their way while the position is)
+    const uint4 lo = ld_global_16b(src + h * p.D + c), hi = ld_global_16b(src + h * p.D + half + c);
+    if (pos < 0) return;  // no token in this row
+    if (i == 0 && (slot >= p.total_slots || pos >= p.max_pos)) std_set_error(STD_DEVERR_BOUNDS);
+    if (pos >= p.max_pos) pos = p.max_pos - 1;
     T* dst;
     if (h < p.Hq) {
       dst = static_cast<T*>(p.q_out) + (static_cast<size_t>(row) * p.Hq + h) * p.D;
