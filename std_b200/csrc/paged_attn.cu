@@ -800,10 +800,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(half == 0 ? &sh.bar_p[s] : &sh.bar_p2[s]);
       }
-      // (the commit in place of the S after the last)
-      if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_s[s][0], ns++ & 1));
       // ---- the item's result ----
-      if (ok && steps > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_o[s], no++ & 1));
+      // (Behind it the commit in place of the S after the last is complete too.  That
+      // is not waited for: the next item's first S may follow it at once.)
+      if (ok && steps > 0) {
+        ++ns;
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_o[s], no++ & 1));
+      }
       if (!ok) break;
       float wa = 1.f, wb = 0.f, m = m_run, l = l_run;
       bool join = false;
