@@ -450,7 +450,7 @@ def paged_update(past_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
     if out is None:
         sizes = (B + 1, B, B, max_tokens, max_tokens)
         cu_q, kv_lens, admitted, slots, positions = torch.empty(
-            sum(sizes), dtype=i32, device=past_lens.device).split_with_sizes(sizes)
+            sum(sizes), dtype=i32, device=past_lens.device).unsafe_split_with_sizes(sizes)  # (no views to keep track of)
     else:
         cu_q, kv_lens, slots, positions, admitted = out
         _paged_check(i32, device, (cu_q, "cu_q", (B + 1,)), (kv_lens, "kv_lens", (B,)),
