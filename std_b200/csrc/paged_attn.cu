@@ -45,16 +45,17 @@
 // not added to, and their V rows are cleared before the product.
 //
 // What bounds it, and what was measured (B200, replayed from a graph; bf16, 28
-// query heads on 4 key heads, D 128 unless said).  Long prompts: a 2048-token
-// chunk over 31K keys 815 us = 1150 TFLOP/s (0.84 of what cuBLAS sustains under
-// the power cap; ncu: tensor pipe 58 % by its own MMAs' time, 71 % counting
-// operand reads; clock 1.65 GHz), an 8192-token prompt 450-530 us as the clock
-// allows.  S in halves costs 1.5 x the shared-memory reads of N=128 but keeps a
-// half of S ready while the other is multiplied: 866 us with one S of 128 columns
-// a step from one issuing thread, 815 with halves and a thread per stream.
+// query heads on 4 key heads, D 128 unless said).  Long prompts: the softmax warps
+// and power; a 2048-token chunk over 31K keys 830 us = 1130 TFLOP/s (0.82 of what
+// cuBLAS sustains under the power cap; 3200 cycles a block of a pair, of which a
+// softmax warp works 2900 and the MMAs need 2560; the clock falls to 1.45 GHz, and
+// in a long run to 1.3: 918 us), an 8192-token prompt 505 us.  S in halves costs 1.5 x
+// the shared-memory reads of N=128 but keeps a half of S ready while the other is
+// multiplied: 866 us with one S of 128 columns a step from one issuing thread, 815
+// with halves and a thread per stream (at the same clock).
 // Decoding: HBM; 64 requests of 100 to 8000 keys 85 us = 5.7 TB/s (0.88 of the
 // measured copy), one request of 131K keys 50 us = 5.4 TB/s, 8 verify blocks of
-// 10 tokens over 33K keys 99 us = 5.4 TB/s; untransposed, the first two took 118
+// 10 tokens over 33K keys 100 us = 5.4 TB/s; untransposed, the first two took 118
 // and 67 us, bound by one warp's softmax of 128 columns for 7 live rows.  Short
 // contexts: latency, 7.5 us for one token and 200 keys, half of it finding the
 // share (2 us) and the first page, key and score (2 us).
@@ -69,7 +70,7 @@ constexpr int PA_THREADS = 384;  // 2 softmax warpgroups; TMA, two MMA and a sch
 constexpr int PA_BN = 128;       // keys per block
 constexpr float PA_RESCALE = 8.0f;  // log2 units
 // Cost of a block in a single and in a pair (measured: 2000 to 2400 cycles and
-// 3700); an item costs PA_OVER blocks more (its queries, first keys and output).
+// 3200 to 3700); an item costs PA_OVER blocks more (its queries, first keys and output).
 constexpr int PA_W1 = 3, PA_W2 = 5, PA_OVER = 3;
 // An item of at most this many blocks is not divided but goes where it begins: a cut
 // would cost a partial and the merge (2 us) to save at most two blocks (2 us), and
@@ -407,8 +408,9 @@ STD_DEV void paged_clear_tail(uint8_t* sV, int last, int thread) {
 
 // Half a step of a whole tile's softmax: 64 columns of S to P, with the row's
 // running m and l.  nvis: visible columns; cut: some row of the warp has fewer than
-// all (known without a vote: 521 -> 515 us for an 8192-token prompt).  bar_next: the barrier (phase parity `next`) after which the
-// stream's products issued so far are complete.  False when a wait ran out.
+// all (known without a vote: 521 -> 515 us for an 8192-token prompt).  bar_next: the
+// barrier (phase parity `next`) after which the stream's products issued so far are
+// complete.  False when a wait ran out.
 template <typename T, int D>
 STD_DEV bool paged_softmax_half(uint32_t tS, uint32_t tO, float sc, int nvis, bool cut, float& m_run, float& l_run,
                                 uint64_t* bar_next, uint32_t next) {
@@ -1227,7 +1229,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           const int per = (walk.items + 31) / 32;
           int sum = 0;
 #pragma unroll 1
-          for (int i = lane * per; i < min((lane + 1) * per, walk.items); ++i) sum += paged_item_cost(p, walk.n, walk.kv, i);
+          for (int i = lane * per; i < min((lane + 1) * per, walk.items); ++i)
+            sum += paged_item_cost(p, walk.n, walk.kv, i);
           const int inc = warp_scan(sum, lane), head = __shfl_sync(0xffffffffu, inc, 31);
           walk.h = off / head;
           off -= walk.h * head;
@@ -1282,12 +1285,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 }
 
 // Joins the pieces of the items that cuts divide: blocks x work at the item that
-// CTA x's share ends inside, so an item of many pieces has many blocks.  out = sum_c w_c o_c / sum_c w_c l_c with w_c =
-// exp2(m_c - max m), in a fixed order of the pieces.  Latency is what counts (a
-// few loads per row, mostly from L2): the grid is one wave, since each wave of
-// blocks costs a memory round trip even where there is nothing to join, and the
-// loads of two rows by two pieces a warp are in flight together, or, for an item
-// of many pieces (a long context), a row's pieces over eight warps.
+// CTA x's share ends inside, so an item of many pieces has many blocks.  out =
+// sum_c w_c o_c / sum_c w_c l_c with w_c = exp2(m_c - max m), in a fixed order of
+// the pieces.  Latency is what counts (a few loads per row, mostly from L2): the
+// grid is one wave, since each wave of blocks costs a memory round trip even where
+// there is nothing to join, and the loads of two rows by two pieces a warp are in
+// flight together, or, for an item of many pieces (a long context), a row's pieces
+// over eight warps.
 constexpr int PM_THREADS = 512;  // (two blocks per SM)
 template <int D>
 struct PagedSum {  // a row's running (m, l, o)
@@ -1473,8 +1477,8 @@ extern "C" int std_paged_attn(const void* q, const void* k_pages, const void* v_
                               const int32_t* cu_q, const int32_t* kv_lens, int T, int B, int Hq, int Hkv, int D,
                               int is_fp16, int num_pages, int page_size, int max_blocks, int causal, float scale,
                               void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
-  if ((D != 64 && D != 128) || T < 0 || B <= 0 || B > STD_PAGED_MAX_REQUESTS || Hkv <= 0 || Hkv > 65535 || Hq <= 0 || Hq % Hkv != 0 ||
-      Hq / Hkv > 128 || num_pages <= 0 || max_blocks <= 0 || !paged_page_ok(page_size))
+  if ((D != 64 && D != 128) || T < 0 || B <= 0 || B > STD_PAGED_MAX_REQUESTS || Hkv <= 0 || Hkv > 65535 || Hq <= 0 ||
+      Hq % Hkv != 0 || Hq / Hkv > 128 || num_pages <= 0 || max_blocks <= 0 || !paged_page_ok(page_size))
     return 1;
   if (!(scale > 0.f) || !(scale < 3.4e38f)) return 1;
   // int32 indexes: keys of a request, slots, 8-row groups of the pool (one page more: the zero fill)
@@ -1489,7 +1493,9 @@ extern "C" int std_paged_attn(const void* q, const void* k_pages, const void* v_
       kv_lens == nullptr || out == nullptr || q == out)
     return 1;
   if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out)) return 1;
-  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 31) != 0 || workspace_bytes < std_paged_attn_workspace_bytes(D)) return 5;
+  if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 31) != 0 ||
+      workspace_bytes < std_paged_attn_workspace_bytes(D))
+    return 5;
   const int G = Hq / Hkv, TQ = 128 / G, TQ_few = stdb::PA_FEW / G;
   CUtensorMap tq, tqf, tk, tv;
   {

@@ -384,7 +384,8 @@ extern "C" int std_paged_rope_append(const void* qkv, int T, int Hq, int Hkv, in
                                      const int32_t* positions, const int32_t* slots, const void* cos_t,
                                      const void* sin_t, int max_pos, void* q_out, void* k_pages, void* v_pages,
                                      int num_pages, int page_size, void* stream) {
-  if (T < 0 || Hq <= 0 || Hkv <= 0 || Hq > 4096 || Hkv > 4096 || (D != 64 && D != 128) || max_pos <= 0 || num_pages <= 0 || !paged_page_ok(page_size))
+  if (T < 0 || Hq <= 0 || Hkv <= 0 || Hq > 4096 || Hkv > 4096 || (D != 64 && D != 128) || max_pos <= 0 ||
+      num_pages <= 0 || !paged_page_ok(page_size))
     return 1;
   if (static_cast<long long>(num_pages) * page_size > 0x7fffffffll) return 1;
   if (T == 0) return 0;
