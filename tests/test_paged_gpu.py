@@ -767,3 +767,44 @@ def test_update_tables_alone(ops):
     assert cu.tolist() == [0, 20, 23] and kv.tolist() == [20, 3] and ok.tolist() == [1, 1]
     assert table[:, :2].tolist() == [[7, 6], [5, -1]] and slots.numel() == pos.numel() == 0
     _no_device_error(ops)
+
+
+def test_queries_beyond_32_bits(ops):
+    """More than 2^31 elements of queries, outputs and qkv rows in one call."""
+    Hq, Hkv, D, page, n, B = 28, 4, 128, 64, 81300, 8  # 2.33e9 elements
+    T, L = B * n, 100
+    blocks = -(-L // page)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    qkv = torch.empty(T, (Hq + 2 * Hkv) * D, dtype=BF, device="cuda")
+    k = torch.randn(B * blocks, Hkv, page, D, generator=g, device="cuda").to(BF)
+    v = torch.randn(B * blocks, Hkv, page, D, generator=g, device="cuda").to(BF)
+    table = torch.arange(B * blocks, dtype=torch.int32, device="cuda").view(B, blocks)
+    rows = [0, 1, n - 1, n, T // 2, T - 36, T - 2, T - 1]
+    qkv.view(T, -1)[rows] = torch.randn(len(rows), qkv.shape[1], generator=g, device="cuda").to(BF)
+    cos, sin = _rope_tables(4, D, BF)
+    q = torch.full((T, Hq, D), 7.0, dtype=BF, device="cuda")
+    pos, slots = torch.full((T,), -1, dtype=torch.int32, device="cuda"), torch.full((T,), -1, dtype=torch.int32, device="cuda")
+    pos[rows] = 0  # (no rotation)
+    slots[T - 1] = (B - 1) * blocks * page + 99
+    ops.paged_rope_append(qkv, pos, slots, cos, sin, q, k, v)
+    new = qkv[rows].view(len(rows), -1, D)
+    assert torch.equal(q[rows], new[:, :Hq]) and (q[[2, n + 1, T - 3]] == 7).all()
+    at = ((B - 1) * blocks + 1, slice(None), 99 - 64)
+    assert torch.equal(k[at], new[-1, Hq:Hq + Hkv]) and torch.equal(v[at], new[-1, Hq + Hkv:])
+    del qkv
+    cu, kv = _i32([n * b for b in range(B + 1)]), _i32([L] * B)
+    out = torch.full_like(q, 3.0)
+    ops.paged_attention(q, k, v, table, cu, kv, causal=False, out=out)
+    for r in rows + [5, T - 7]:
+        b = r // n
+        kk = k[table[b].long()].permute(1, 0, 2, 3).reshape(Hkv, -1, D)[:, :L].double().repeat_interleave(7, 0)
+        vv = v[table[b].long()].permute(1, 0, 2, 3).reshape(Hkv, -1, D)[:, :L].double().repeat_interleave(7, 0)
+        s = torch.einsum("hd,hld->hl", q[r].double(), kk) / math.sqrt(D)
+        p = torch.softmax(s, -1)
+        ref, A = torch.einsum("hl,hld->hd", p, vv), torch.einsum("hl,hld->hd", p, vv.abs())
+        assert ((out[r].double() - ref).abs() <= 1.02 * 2.0 ** -8 * (ref.abs() + A)).all(), r
+    ops.paged_attention(q, k, v, table, cu, kv, out=out)  # causal: the last 100 tokens of each see keys
+    seen = [n - L, n - 1, T - L, T - 1]
+    assert (out[[0, n - L - 1, T - L - 1]] == 0).all()
+    assert torch.equal(out[[n - L, T - L]][:, ::7], v[table[[0, B - 1], 0].long(), :, 0]) and (out[seen] != 0).any(-1).all()
+    _no_device_error(ops)
