@@ -98,6 +98,15 @@ constexpr int PA_FEW = 32;
 // long run: none 972 us, every 8th 950, 4th 947, 3rd 942; every 2nd is slower again).
 constexpr int PA_POLY = 3;
 
+// Steps of a stream after which its O is added to a sum in global memory (the slot
+// that the item's partial takes, or would take) and started anew.  The tensor core
+// cuts its 32-bit sums off instead of rounding them, so a sum of same-signed values
+// lags by about 2^-24 of itself with each 16 keys: without this 4.5e-3 over 2^20 keys
+// in one CTA, more than half a step of bf16; with it below 3e-4 at any length (8
+// verify blocks over 33K keys, which never come here, 1 % slower for the longer code,
+// the 2048-token chunk the same).
+constexpr int PA_FLUSH = 512;
+
 // What a CTA leaves for the merge about the item that its share ends inside.
 struct PagedSplit {
   int first_cta, last_cta;  // where the item's pieces are; last < 0: nothing to merge
@@ -271,6 +280,7 @@ struct PagedShared {
       alignas(16) float up[2][PA_FEW];     // by how much m was raised last
     };
   };
+  float m_sum[2][PA_FEW];  // few rows: m of each stream's sum in global memory
   alignas(16) int flag[2][2][4];  // few rows: a vote per warp, by step parity
   PagedPiece piece[PA_PIECES];
   uint32_t tmem;
@@ -406,6 +416,40 @@ STD_DEV void paged_clear_tail(uint8_t* sV, int last, int thread) {
   fence_async_smem();
 }
 
+// A stream's O of whole tiles and its row's sum in global memory: sum = f sum + O,
+// O = 0 (begin: there is no sum yet), f = 2^(m of the sum - m of O); or, to end with,
+// O += f sum.  For a warp whose products are at rest.  (A call: inlined, it cost the
+// loops around it 1 %.)
+template <int D>
+__device__ __noinline__ void paged_flush(uint32_t tO, float* sum, float f, bool begin, bool end) {
+  tc_fence_after();
+  uint32_t o[16];
+#pragma unroll 1
+  for (int c = 0; c < D; c += 16) {
+    tmem_ld16(tO + c, o);
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+      float4* at = reinterpret_cast<float4*>(sum + c + j);
+      float4 v = make_float4(__uint_as_float(o[j]), __uint_as_float(o[j + 1]), __uint_as_float(o[j + 2]),
+                             __uint_as_float(o[j + 3]));
+      if (!begin) {
+        const float4 a = *at;
+        v = make_float4(fmaf(a.x, f, v.x), fmaf(a.y, f, v.y), fmaf(a.z, f, v.z), fmaf(a.w, f, v.w));
+      }
+      if (!end) {
+        *at = v;
+        v = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      o[j] = __float_as_uint(v.x), o[j + 1] = __float_as_uint(v.y);
+      o[j + 2] = __float_as_uint(v.z), o[j + 3] = __float_as_uint(v.w);
+    }
+    tmem_st16(tO + c, o);
+  }
+  tmem_wait_st();
+  tc_fence_before();
+}
+
 // Half a step of a whole tile's softmax: 64 columns of S to P, with the row's
 // running m and l.  nvis: visible columns; cut: some row of the warp has fewer than
 // all (known without a vote: 521 -> 515 us for an 8192-token prompt).  bar_next: the
@@ -455,7 +499,7 @@ STD_DEV bool paged_softmax_half(uint32_t tS, uint32_t tO, float sc, int nvis, bo
   // a row that has seen no key yet keeps P = 2^-inf = 0
   const float nm = m_run == -INFINITY ? 0.f : -m_run;
   const uint64_t sc2 = f2_make(sc, sc), nm2 = f2_make(nm, nm);
-  uint64_t l2[2] = {f2_make(l_run, 0.f), f2_make(0.f, 0.f)};
+  uint64_t l2[2] = {f2_make(0.f, 0.f), f2_make(0.f, 0.f)};
   uint32_t pk[N / 2];
 #pragma unroll
   for (int j = 0; j < N / 2; ++j) {
@@ -477,7 +521,7 @@ STD_DEV bool paged_softmax_half(uint32_t tS, uint32_t tO, float sc, int nvis, bo
   const float2 l = f2_split(f2_add(l2[0], l2[1]));
   // A NaN or infinite score makes its row NaN: it has left a NaN here or, through
   // ex2_fma2, FLT_MAX or more; sums of numbers stay below 2^31 2^PA_RESCALE.
-  l_run = l.x + l.y;
+  l_run += l.x + l.y;
   if (!(l_run < 1e30f)) l_run = NAN;
   return true;
 }
@@ -529,6 +573,33 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
     if (lane == 0) mbar_arrive(&sh.bar_group[s]);
     return __all_sync(0xffffffffu, mbar_wait(&sh.bar_group[s], ng++ & 1));
   };
+  float* sum = p.ws_o + (static_cast<size_t>(piece.slot < 0 ? 2 * blockIdx.x + 1 : piece.slot) * 256 + s * 128) * D + key;
+  // paged_flush for O^T: thread = head dim, a column per row
+  auto flush = [&](bool begin, bool end) -> bool {
+    uint32_t o[16];
+#pragma unroll 1
+    for (int c = 0; c < N; c += 16) {
+      tmem_ld16(tO + c, o);
+      tmem_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        float v = __uint_as_float(o[j]);
+        if (key < D) {
+          float* at = sum + static_cast<size_t>(c + j) * D;
+          if (!begin) v = fmaf(*at, ex2_approx(sh.m_sum[s][c + j] - sh.ref[s][c + j]), v);
+          if (!end) *at = v;
+        }
+        o[j] = end ? __float_as_uint(v) : 0u;
+      }
+      tmem_st16(tO + c, o);
+    }
+    tmem_wait_st();
+    tc_fence_before();
+    if (end) return true;
+    if (!group_sync()) return false;
+    if (key < N) sh.m_sum[s][key] = sh.ref[s][key];
+    return true;  // (m_sum is read again after more group syncs)
+  };
   float l[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) l[n] = 0.f;
@@ -536,6 +607,7 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
   for (int k = 0; k < steps; ++k, ++ns) {
     if (!__all_sync(0xffffffffu, mbar_wait(&sh.bar_s[s][0], ns & 1))) return false;
     tc_fence_after();
+    if (k > 0 && k % PA_FLUSH == 0 && !flush(k == PA_FLUSH, false)) return false;  // (O is at rest)
     float y[N];
     tmem_ld_cols<N>(tS, reinterpret_cast<uint32_t*>(y));
     tmem_wait_ld();
@@ -615,6 +687,10 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
   }
   if (steps > 0) {
     if (!__all_sync(0xffffffffu, mbar_wait(&sh.bar_o[s], no++ & 1))) return false;
+    if (steps > PA_FLUSH) {
+      tc_fence_after();
+      flush(false, true);
+    }
     const int base = warp_reduce_rows<N>(l, lane, [](float a, float b) { return a + b; });
     red(s, w, base) = l[0];
     fence_async_smem();  // (a TMA load may write here next)
@@ -773,37 +849,56 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
       const int limit = p.causal ? min(piece.limit, piece.first + t) : piece.limit;
       const int all_see = __reduce_min_sync(0xffffffffu, limit);  // keys that all rows of the warp see
       const int steps = pair ? nblk : (nblk - s + 1) >> 1;
-      float m_run = -INFINITY, l_run = 0.f;
+      float m_run = -INFINITY, l_run = 0.f, m_sum = -INFINITY, l_sum = 0.f;
+      // O and l to their sums: begin: the first time; end: and back
+      auto flush = [&](bool begin, bool end) {
+        float* sum =
+            p.ws_o + (static_cast<size_t>(piece.slot < 0 ? 2 * cta + 1 : piece.slot) * 256 + s * 128 + r) * D;
+        const float f = m_sum == m_run ? 1.f : exp2f(m_sum - m_run);
+        paged_flush<D>(tO, sum, f, begin, end);
+        l_sum = fmaf(l_sum, f, l_run);
+        l_run = end ? l_sum : 0.f;
+        m_sum = m_run;
+      };
 #pragma unroll 1
-      for (int h = 0; ok && h < 2 * steps; ++h) {  // half steps
-        const int half = h & 1, k = h >> 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_s[s][half], (half == 0 ? ns : ns1) & 1));
-        if (!ok) break;
-        const int k0 = (piece.j0 + (pair ? k : 2 * k + s)) * PA_BN, left = piece.limit - k0;
-        if (half == 0) {
-          ++ns;
-          if (left < PA_BN && (left & 15) != 0) {
-            // the last block, which ends inside a 16-key step (both streams of a pair
-            // clear its rows, each before its own product)
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_tail[s], ntail++ & 1));
-            if (!ok) break;
-            paged_clear_tail<D>(sV, left, r);
-            __syncwarp();
-          }
-        } else {
-          ++ns1;
-        }
-        if (live) {
-          tc_fence_after();
-          // (limit - k0: visible keys of this block.)  The products so far are complete
-          // once the other half's next S is: it was issued after the last of them.
-          ok = paged_softmax_half<T, D>(tS + half * (PA_BN / 2), tO, sc, limit - k0 - half * (PA_BN / 2),
-                                        k0 + (half + 1) * (PA_BN / 2) > all_see, m_run, l_run,
-                                        &sh.bar_s[s][half ^ 1], half == 0 ? ns1 : ns);
+      for (int h = 0, h_end = 0; ok && h < 2 * steps;) {
+        if (h > 0 && live) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_s[s][1], ns1 & 1));  // O at rest
           if (!ok) break;
+          flush(h == 2 * PA_FLUSH, false);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(half == 0 ? &sh.bar_p[s] : &sh.bar_p2[s]);
+        h_end = min(2 * steps, h + 2 * PA_FLUSH);
+#pragma unroll 1
+        for (; ok && h < h_end; ++h) {  // half steps
+          const int half = h & 1, k = h >> 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_s[s][half], (half == 0 ? ns : ns1) & 1));
+          if (!ok) break;
+          const int k0 = (piece.j0 + (pair ? k : 2 * k + s)) * PA_BN, left = piece.limit - k0;
+          if (half == 0) {
+            ++ns;
+            if (left < PA_BN && (left & 15) != 0) {
+              // the last block, which ends inside a 16-key step (both streams of a pair
+              // clear its rows, each before its own product)
+              ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_tail[s], ntail++ & 1));
+              if (!ok) break;
+              paged_clear_tail<D>(sV, left, r);
+              __syncwarp();
+            }
+          } else {
+            ++ns1;
+          }
+          if (live) {
+            tc_fence_after();
+            // (limit - k0: visible keys of this block.)  The products so far are complete
+            // once the other half's next S is: it was issued after the last of them.
+            ok = paged_softmax_half<T, D>(tS + half * (PA_BN / 2), tO, sc, limit - k0 - half * (PA_BN / 2),
+                                          k0 + (half + 1) * (PA_BN / 2) > all_see, m_run, l_run,
+                                          &sh.bar_s[s][half ^ 1], half == 0 ? ns1 : ns);
+            if (!ok) break;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(half == 0 ? &sh.bar_p[s] : &sh.bar_p2[s]);
+        }
       }
       // ---- the item's result ----
       // (Behind it the commit in place of the S after the last is complete too.  That
@@ -813,6 +908,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_o[s], no++ & 1));
       }
       if (!ok) break;
+      if (steps > PA_FLUSH && live) flush(false, true);
       float wa = 1.f, wb = 0.f, m = m_run, l = l_run;
       bool join = false;
       if (!pair) {

@@ -808,3 +808,42 @@ def test_queries_beyond_32_bits(ops):
     assert (out[[0, n - L - 1, T - L - 1]] == 0).all()
     assert torch.equal(out[[n - L, T - L]][:, ::7], v[table[[0, B - 1], 0].long(), :, 0]) and (out[seen] != 0).any(-1).all()
     _no_device_error(ops)
+
+
+@pytest.mark.parametrize("new,D,dtype", [(1, 64, FP), (4, 128, FP), (12, 64, FP), (36, 64, FP), (36, 128, BF)])
+def test_sums_over_a_million_keys(ops, new, D, dtype):
+    """2^20 keys in one CTA (few rows, one tile, a pair): the sums do not drift.  150
+    requests on the same pages, the later pages' scores above the earlier ones'.
+
+    A CTA's stream adds 16 keys at a time to a 32-bit sum, cut off (2^-23 of it each
+    time at most), starts anew every 512 blocks of 128 keys and rounds once there:
+    4096 2^-23 + 32 2^-24 = 4.9e-4 relative, of same-signed values; l lags by 64 per
+    2^20 / 128 / 2 and thread at most, 2^-24 each and both ways: 2.5e-4.  Besides, the
+    rounding of the output, e / 2, and of the probabilities: e / 2 of sum p |v| = ref,
+    in full, as a key that comes again has the same error each time (a few of the 1024
+    keys can hold nearly all of a row's weight, so nothing averages out)."""
+    L, page, G = 1 << 20, 256, 7
+    g = torch.Generator(device="cuda").manual_seed(new)
+    k = torch.randn(4, 1, page, D, generator=g, device="cuda")
+    k[:2] *= 0.2
+    k = k.to(dtype)
+    v = (torch.rand(4, 1, page, D, generator=g, device="cuda") + 0.5).to(dtype)
+    v[..., 0] = 1
+    blocks, B = L // page, 150
+    ids = torch.arange(blocks, device="cuda")
+    row = torch.where(ids < blocks * 5 // 8, ids % 2, 2 + ids % 2).int()
+    q = (3 * torch.randn(B * new, G, D, generator=g, device="cuda")).to(dtype)
+    lse = torch.empty(B * new, G, device="cuda")
+    cu, kv = torch.arange(0, B * new + 1, new, device="cuda").int(), torch.full((B,), L - 100, device="cuda").int()
+    out = ops.paged_attention(q, k, v, row.expand(B, -1).contiguous(), cu, kv, causal=False, lse=lse).double()
+    count = torch.stack([(row == i).sum() for i in range(4)]).double()[:, None].expand(4, page).clone()
+    count[row[-1].long(), page - 100:] -= 1
+    s = torch.einsum("nhd,pkd->nhpk", q.double(), k[:, 0].double()) / math.sqrt(D)
+    m = s.amax((-1, -2), keepdim=True)
+    w = torch.exp(s - m) * count
+    l = w.sum((-1, -2))
+    ref = torch.einsum("nhpk,pkd->nhd", w, v[:, 0].double()) / l[..., None]
+    e = torch.finfo(dtype).eps
+    assert ((out - ref).abs() <= (7.4e-4 + e / 2 + e / 2) * ref).all(), ((out - ref).abs() / ref).max().item()
+    assert ((lse.double() - (l.log() + m[..., 0, 0])).abs() <= 2.5e-4 + 30 * 2.0 ** -22).all()
+    _no_device_error(ops)
