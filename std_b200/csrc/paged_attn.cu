@@ -245,7 +245,7 @@ STD_DEV void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, 
 template <int ST>
 struct PagedShared {
   // mbarriers, by the arrivals that complete a phase
-  static constexpr int BARS_1 = 12 + ST + PA_PIECES, BARS_2 = BARS_1 + ST, BARS_3 = BARS_2 + 2,
+  static constexpr int BARS_1 = 14 + ST + PA_PIECES, BARS_2 = BARS_1 + ST, BARS_3 = BARS_2 + 2,
                        BARS_4 = BARS_3 + 8, BARS = BARS_4 + PA_PIECES;
   union {
     uint64_t bars[BARS];
@@ -253,6 +253,7 @@ struct PagedShared {
       // one
       uint64_t bar_q_full[2];                  // query slots
       uint64_t bar_s[2][2], bar_o[2];          // per stream: S's halves there, O complete
+      uint64_t bar_half[2];                    // whole tiles: the product of an item's last first half done
       uint64_t bar_tail[2], bar_end[2];        // a tail's V there; all MMAs done
       uint64_t bar_full[ST];                   // K/V ring
       uint64_t bar_piece[PA_PIECES];
@@ -823,7 +824,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const int rt = r / p.G, rg = r % p.G;  // token and head of this row in its tile
     const float sc = p.scale_log2;
     uint32_t npiece = 0, ns = 0, no = 0, nj = 0, ng = 0;  // pieces, steps, results, joins, group syncs so far
-    uint32_t ns1 = 0;                              // steps' second halves
+    uint32_t ns1 = 0, na = 0;                      // steps' second halves, whole-tile items
     uint32_t nq = 0, ntail = 0, nld = 0;           // query tiles, tails cleared, loads so far
     bool ok = true;
     PagedPiece piece;
@@ -890,10 +891,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
           if (live) {
             tc_fence_after();
             // (limit - k0: visible keys of this block.)  The products so far are complete
-            // once the other half's next S is: it was issued after the last of them.
+            // once the other half's next S is: it was issued after the last of them.  Behind
+            // the last step there is none, and bar_half takes its place.
+            const bool at_end = h + 1 == 2 * steps;
             ok = paged_softmax_half<T, D>(tS + half * (PA_BN / 2), tO, sc, limit - k0 - half * (PA_BN / 2),
                                           k0 + (half + 1) * (PA_BN / 2) > all_see, m_run, l_run,
-                                          &sh.bar_s[s][half ^ 1], half == 0 ? ns1 : ns);
+                                          at_end ? &sh.bar_half[s] : &sh.bar_s[s][half ^ 1],
+                                          at_end ? na : (half == 0 ? ns1 : ns));
             if (!ok) break;
           }
           __syncwarp();
@@ -901,12 +905,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
       }
       // ---- the item's result ----
-      // (Behind it the commit in place of the S after the last is complete too.  That
-      // is not waited for: the next item's first S may follow it at once.)
-      if (ok && steps > 0) {
-        ++ns;
-        ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_o[s], no++ & 1));
-      }
+      // Every warp waits for every phase of both barriers: nothing says that two commits
+      // arrive in the order of their issue, and a wait by parity must not fall two behind.
+      // (The next phase of each needs this warp's next P, so neither can be two ahead.)
+      if (ok && steps > 0)
+        ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_half[s], na++ & 1)) &&
+             __all_sync(0xffffffffu, mbar_wait(&sh.bar_o[s], no++ & 1));
       if (!ok) break;
       if (steps > PA_FLUSH && live) flush(false, true);
       float wa = 1.f, wb = 0.f, m = m_run, l = l_run;
@@ -1060,9 +1064,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             ++kv;
         }
       }
-      // never leave a copy in flight
-      for (uint32_t c = nld < ST ? 0 : nld - ST; c < nld; ++c) mbar_wait(&sh.bar_full[c % ST], (c / ST) & 1);
-      for (uint32_t c = nq < 2 ? 0 : nq - 2; c < nq; ++c) mbar_wait(&sh.bar_q_full[c & 1], (c >> 1) & 1);
+      // never leave a copy in flight, nor a commit that has yet to arrive on a barrier
+      for (uint32_t c = nld < ST ? 0 : nld - ST; c < nld; ++c) {
+        mbar_wait(&sh.bar_full[c % ST], (c / ST) & 1);
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_empty[c % ST], (c / ST) & 1));
+      }
+      for (uint32_t c = nq < 2 ? 0 : nq - 2; c < nq; ++c) {
+        mbar_wait(&sh.bar_q_full[c & 1], (c >> 1) & 1);
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&sh.bar_q_empty[c & 1], (c >> 1) & 1));
+      }
     } else if (warp < 11) {
       // ---------------- MMA issuers: one thread per stream ----------------
       // A stream's S and P V go out in order from one thread, which is what lets S
@@ -1214,7 +1224,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                   tc_fence_after();
                   s_half(at, 0);
                 } else {
-                  umma_commit(&sh.bar_s[s][0]);  // for a second half that rescales O
+                  umma_commit(&sh.bar_half[s]);  // for a second half that rescales O
                 }
                 ok = mbar_wait(&sh.bar_p2[s], np2++ & 1);
                 if (!ok) break;
