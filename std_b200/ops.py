@@ -410,6 +410,22 @@ def _paged_device(t: torch.Tensor, name: str) -> int:
     return device
 
 
+def _paged_own(names: str, *tensors: torch.Tensor) -> None:
+    """Memory that a call took for itself.  Captured into a graph it has to stay the
+    graph's, as it does under torch.cuda.graph (from the graph's own pool).  A capture
+    that torch did not begin (a loop or branch body, std_capture_while_begin and
+    std_capture_if_begin) gets it from the general pool instead, which would hand it
+    to others while the graph still writes it: refused."""
+    if not torch._C._cuda_isCurrentStreamCapturing() or torch.cuda.get_allocator_backend() != "native":
+        return
+    segments = torch.cuda.memory_snapshot(include_traces=False)
+    for at in (t.data_ptr() for t in tensors if t.numel() > 0):
+        pools = [tuple(s["segment_pool_id"]) for s in segments if s["address"] <= at < s["address"] + s["total_size"]]
+        if not pools or pools[0] == (0, 0):
+            raise RuntimeError(f"a capture that torch.cuda.graph did not begin (a graph's loop or branch body) needs "
+                               f"{names}: memory allocated here would not stay with the graph")
+
+
 def _paged_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtype, device: int):
     if k_pages.dim() != 4:
         raise ValueError("k_pages must be [num_pages, Hkv, page_size, D]")
@@ -434,7 +450,8 @@ def paged_update(past_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
     shorter past_lens rolls a request back.  Returns (cu_q [B + 1], kv_lens [B],
     slots [max_tokens], positions [max_tokens], admitted [B]); a request that the
     list cannot serve has admitted 0, kv_lens 0 and slots -1.  `out` gives the
-    five result tensors (a captured graph's static buffers)."""
+    five result tensors (a captured graph's static buffers; the captured body of a
+    loop or branch needs it)."""
     device = _paged_device(past_lens, "past_lens")
     B, i32 = past_lens.numel(), torch.int32
     if B < 1:
@@ -449,8 +466,9 @@ def paged_update(past_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
                  (free_pages, "free_pages", (num_pages,)), (n_free, "n_free", (1,)))
     if out is None:
         sizes = (B + 1, B, B, max_tokens, max_tokens)
-        cu_q, kv_lens, admitted, slots, positions = torch.empty(
-            sum(sizes), dtype=i32, device=past_lens.device).unsafe_split_with_sizes(sizes)  # (no views to keep track of)
+        room = torch.empty(sum(sizes), dtype=i32, device=past_lens.device)
+        _paged_own("out=", room)
+        cu_q, kv_lens, admitted, slots, positions = room.unsafe_split_with_sizes(sizes)  # (no views to keep track of)
     else:
         cu_q, kv_lens, slots, positions, admitted = out
         _paged_check(i32, device, (cu_q, "cu_q", (B + 1,)), (kv_lens, "kv_lens", (B,)),
@@ -487,9 +505,27 @@ def paged_rope_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.T
     return q_out
 
 
+def _paged_workspace_bytes(D: int) -> int:
+    nb = _PAGED_WS_BYTES.get(D)
+    if nb is None:
+        nb = _PAGED_WS_BYTES[D] = _lib.query("std_paged_attn_workspace_bytes", D)
+    return nb
+
+
+def paged_attention_workspace(head_dim: int, device: Optional[torch.device] = None) -> torch.Tensor:
+    """A workspace for paged_attention calls of this head dim (64 or 128) on one
+    stream, or captured into one graph: calls that may run at the same time need
+    one each.  device defaults to the current one."""
+    nb = _paged_workspace_bytes(int(head_dim))
+    if nb == 0:
+        raise ValueError(f"head dim must be 64 or 128, got {head_dim}")
+    return torch.empty(nb, dtype=torch.uint8, device="cuda" if device is None else device)
+
+
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
                     cu_q: torch.Tensor, kv_lens: torch.Tensor, causal: bool = True, scale: Optional[float] = None,
-                    out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None):
+                    out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                    workspace: Optional[torch.Tensor] = None):
     """Attention of each request's new tokens over its paged cache.
 
     q [T, Hq, D]: request b's tokens are rows cu_q[b] .. cu_q[b+1] - 1 (cu_q [B +
@@ -498,7 +534,10 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     kv_len - n + t (causal) or all kv_len.  bf16 or fp16; any Hq / Hkv up to 128.
     scale defaults to 1 / sqrt(D).  out [T, Hq, D], lse [T, Hq] fp32 (optional).
     Rows that see no key give 0 and -inf; rows outside every request are left
-    as they were (uninitialised in an `out` made here)."""
+    as they were (uninitialised in an `out` made here).  workspace (optional): a
+    buffer of paged_attention_workspace, which no other call may use before this
+    one has run; one kept by the caller serves a whole sequence of calls.  The
+    captured body of a loop or branch needs `out` and `workspace`."""
     device = _paged_device(q, "q")
     dtype = q.dtype
     if dtype not in _PAGED_DTYPES:
@@ -516,18 +555,28 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 0.0 < scale < 3e38:
         raise ValueError(f"scale must be positive and finite, got {scale}")
+    made = ()  # here
     if out is None:
         out = torch.empty_like(q)
+        made = (out,)
     else:
         _paged_check(dtype, device, (out, "out", (T, Hq, D)))
     if lse is not None:
         _paged_check(torch.float32, device, (lse, "lse", (T, Hq)))
-    # Of this call alone: the caching allocator hands it out in stream order, and
-    # under capture from the graph's own pool, so no two calls or graphs share it.
-    nb = _PAGED_WS_BYTES.get(D)
-    if nb is None:
-        nb = _PAGED_WS_BYTES[D] = _lib.query("std_paged_attn_workspace_bytes", D)
-    ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
+    nb = _paged_workspace_bytes(D)
+    if workspace is None:
+        # Of this call alone: the caching allocator hands it out in stream order, and
+        # under torch.cuda.graph from the graph's own pool, so no two calls or graphs
+        # share it.
+        ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
+        made += (ws,)
+    else:
+        ws = workspace
+        _paged_check(torch.uint8, device, (ws, "workspace", ws.shape))
+        if ws.numel() < nb or ws.data_ptr() % 32 != 0:
+            raise ValueError(f"workspace must have at least {nb} bytes and begin at a multiple of 32")
+    if made:
+        _paged_own("out= and workspace=", *made)
     _lib.call("std_paged_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
               cu_q.data_ptr(), kv_lens.data_ptr(), T, B, Hq, Hkv, D, 1 if dtype == torch.float16 else 0, num_pages,
               page, width, 1 if causal else 0, scale, out.data_ptr(), _p(lse), ws.data_ptr(), nb, _stream_of(device))

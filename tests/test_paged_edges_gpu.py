@@ -1,6 +1,7 @@
 """GPU: edges of the paged K/V cache operators: maxima that rise inside an item's
 last block, captured loop bodies, empty steps, infinite scores, idle requests, long
 prompts.  Tolerances as derived in test_paged_gpu."""
+import ctypes
 import math
 
 import pytest
@@ -47,4 +48,102 @@ def test_maximum_rises_in_every_half_block(ops, D, dtype, tail):
         out = x.call(ops, causal, lse=lse)
         x.check(out, lse, causal)
         assert torch.equal(x.call(ops, causal), out)
+    _no_device_error(ops)
+
+
+# ------------------------------------------------------------------ workspaces and captured bodies
+def test_workspace_of_the_caller(ops):
+    """The same bits with a workspace kept over calls of different shapes; what is too
+    small, misaligned or of another type is refused."""
+    calls = [Paged([(4000, 1), (3000, 3)], 28, 4, 128, 16, BF, seed=1), Paged([(100, 900)], 8, 8, 128, 32, FP, seed=2),
+             Paged([(9000, 1)], 28, 4, 128, 64, BF, seed=3)]
+    ws = ops.paged_attention_workspace(128)
+    for x in calls + calls:
+        assert torch.equal(x.call(ops, workspace=ws), x.call(ops))
+    x = calls[0]
+    with pytest.raises(ValueError, match="workspace"):
+        x.call(ops, workspace=ws[:-1])
+    with pytest.raises(ValueError, match="workspace"):
+        x.call(ops, workspace=torch.empty(ws.numel() + 16, dtype=torch.uint8, device="cuda")[16:])
+    with pytest.raises(RuntimeError, match="workspace"):
+        x.call(ops, workspace=ws.view(torch.int32))
+    with pytest.raises(RuntimeError, match="workspace"):
+        x.call(ops, workspace=ws.cpu())
+    with pytest.raises(ValueError, match="head dim"):
+        ops.paged_attention_workspace(96)
+    _no_device_error(ops)
+
+
+def _loop(body, done, count, limit):
+    """`body` as the loop body of a graph being captured, run until done is set."""
+    from std_b200 import _lib
+
+    inner, h = _lib.capture_stream("while_body"), ctypes.c_ulonglong(0)
+    _lib.call("std_capture_while_begin", torch.cuda.current_stream().cuda_stream, inner.cuda_stream, done.data_ptr(),
+              done.numel(), count.data_ptr(), ctypes.byref(h), None)
+    with torch.cuda.stream(inner):
+        body()
+    _lib.call("std_capture_while_end", inner.cuda_stream, h.value, done.data_ptr(), done.numel(), count.data_ptr(), limit)
+
+
+def test_captured_loop_bodies(ops):
+    """A loop body captures the calls with buffers of the caller's; its replays touch no
+    memory that was given to others since.  Without them it refuses, as they would
+    come from memory that does not stay with the graph."""
+    a, b = Paged([(9000, 1), (40, 30)], 28, 4, 128, 16, BF, seed=1), Paged([(7000, 2), (50, 300)], 28, 4, 128, 64, BF, seed=2)
+    want = [a.call(ops), b.call(ops)]
+    done, graphs, kept = _i32([0]), [], []
+    for x in (a, b):
+        out, ws, count = torch.zeros_like(x.q), ops.paged_attention_workspace(128), _i32([0])
+        lens = [n for _, n in x.pairs]
+        past, new, held, n_free = _i32([p for p, _ in x.pairs]), _i32(lens), _i32([0] * 2), _i32([1000])
+        table, free = torch.full((2, 800), -1, dtype=torch.int32, device="cuda"), torch.arange(1000, device="cuda").int()
+        steps = [torch.zeros(n, dtype=torch.int32, device="cuda") for n in (3, 2, sum(lens), sum(lens), 2)]
+
+        def body():
+            ops.paged_update(past, new, table, held, free, n_free, 16, sum(lens), out=steps)
+            x.call(ops, out=out, workspace=ws)
+            for kw in (dict(), dict(out=out), dict(workspace=ws)):
+                with pytest.raises(RuntimeError, match="workspace="):
+                    x.call(ops, **kw)
+            with pytest.raises(RuntimeError, match="out="):
+                ops.paged_update(past, new, table, held, free, n_free, 16, sum(lens))
+
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            _loop(body, done, count, 3)
+        graphs.append(g)
+        kept.append((out, ws, count, steps, x.kv_lens, x.cu, past, new, table, held, free, n_free))
+    torch.cuda.empty_cache()
+    others = [torch.full((24 << 20,), 7, dtype=torch.uint8, device="cuda") for _ in range(12)]
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        for out, *_ in kept:
+            out.zero_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, (s1, s2)):  # both loops at once
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for (out, _, count, steps, kv, cu, *_), w in zip(kept, want):
+            assert torch.equal(out, w) and count.item() == 3
+            assert torch.equal(steps[0], cu) and torch.equal(steps[1], kv)
+        assert all((o == 7).all() for o in others)
+    _no_device_error(ops)
+
+
+def test_graphs_of_torch_need_no_workspace(ops):
+    """Under torch.cuda.graph a call's own memory stays with the graph."""
+    x = Paged([(9000, 1), (40, 300)], 28, 4, 128, 16, BF, seed=1)
+    want, g = x.call(ops), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        out = x.call(ops)
+    torch.cuda.empty_cache()
+    others = [torch.full((24 << 20,), 7, dtype=torch.uint8, device="cuda") for _ in range(6)]
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        assert torch.equal(out, want) and all((o == 7).all() for o in others)
     _no_device_error(ops)
