@@ -147,3 +147,45 @@ def test_graphs_of_torch_need_no_workspace(ops):
         g.replay()
         assert torch.equal(out, want) and all((o == 7).all() for o in others)
     _no_device_error(ops)
+
+
+# ------------------------------------------------------------------ idle requests
+@pytest.mark.parametrize("B", [33, 64, 2047, 8192])
+def test_mostly_idle_batches(ops, B):
+    """Requests without new tokens between those that have some, in runs of all lengths:
+    the same rows as without them."""
+    lens = {0: (700, 1), 1: (90, 20), B // 2: (40, 1), B - 33: (300, 3), B - 2: (1200, 2), B - 1: (64, 5)}
+    lens = dict(sorted(lens.items()))  # (rows come in request order)
+    x = Paged(list(lens.values()), 28, 4, 128, 16, BF, seed=B)
+    x.check(x.call(ops), None)
+    cu, kv, at = [0], [0] * B, dict(zip(lens, range(len(lens))))
+    table = torch.full((B, x.table.shape[1]), -1, dtype=torch.int32, device="cuda")
+    for b in range(B):
+        cu.append(cu[-1] + (lens[b][1] if b in lens else 0))
+        if b in lens:
+            kv[b], table[b] = sum(lens[b]), x.table[at[b]]
+        elif b % 3 == 0:
+            kv[b] = 50  # (keys, but no new tokens)
+    out = ops.paged_attention(x.q, x.k, x.v, table, _i32(cu), _i32(kv))
+    assert torch.equal(out, x.call(ops))
+    _no_device_error(ops)
+
+
+def test_idle_requests_are_passed_quickly(ops):
+    """8192 requests, two at each end with a token: every CTA reads all lengths twice (about
+    0.1 ms), whatever lies between its requests (passed one by one: 1.6 ms)."""
+    from std_b200.timing import graph_time_us
+
+    x = Paged([(999, 1)] * 4, 28, 4, 128, 64, BF)
+    times = []
+    for ids in ([0, 1, 2, 3], [0, 1, 8190, 8191]):
+        new, kv = torch.zeros(8192, dtype=torch.int32), torch.zeros(8192, dtype=torch.int32)
+        new[ids], kv[ids] = 1, 1000
+        table = torch.full((8192, x.table.shape[1]), -1, dtype=torch.int32, device="cuda")
+        table[ids] = x.table
+        cu = torch.cat([torch.zeros(1), new.cumsum(0)]).int().cuda()
+        kv, out = kv.cuda(), torch.empty_like(x.q)
+        times.append(graph_time_us([lambda: ops.paged_attention(x.q, x.k, x.v, table, cu, kv, out=out)]))
+        x.check(out, None)
+    assert times[1] < 3 * times[0], times
+    _no_device_error(ops)
