@@ -405,18 +405,18 @@ def _paged_device(t: torch.Tensor, name: str) -> int:
     device = t.get_device()
     if device < 0:
         raise RuntimeError(f"{name} must be a CUDA tensor (no CPU path)")
-    if device != torch.cuda.current_device():
+    if device != torch._C._cuda_getDevice():  # (torch.cuda.current_device without its check that CUDA is up)
         raise RuntimeError(f"{name} is on {t.device}, but cuda:{torch.cuda.current_device()} is the current device")
     return device
 
 
 def _paged_own(names: str, *tensors: torch.Tensor) -> None:
-    """Memory that a call took for itself.  Captured into a graph it has to stay the
-    graph's, as it does under torch.cuda.graph (from the graph's own pool).  A capture
+    """Memory that a call took for itself while its stream is being captured: it has
+    to stay the graph's, as it does under torch.cuda.graph (from the graph's own pool).  A capture
     that torch did not begin (a loop or branch body, std_capture_while_begin and
     std_capture_if_begin) gets it from the general pool instead, which would hand it
     to others while the graph still writes it: refused."""
-    if not torch._C._cuda_isCurrentStreamCapturing() or torch.cuda.get_allocator_backend() != "native":
+    if torch.cuda.get_allocator_backend() != "native":
         return
     segments = torch.cuda.memory_snapshot(include_traces=False)
     for at in (t.data_ptr() for t in tensors if t.numel() > 0):
@@ -467,7 +467,8 @@ def paged_update(past_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
     if out is None:
         sizes = (B + 1, B, B, max_tokens, max_tokens)
         room = torch.empty(sum(sizes), dtype=i32, device=past_lens.device)
-        _paged_own("out=", room)
+        if torch._C._cuda_isCurrentStreamCapturing():
+            _paged_own("out=", room)
         cu_q, kv_lens, admitted, slots, positions = room.unsafe_split_with_sizes(sizes)  # (no views to keep track of)
     else:
         cu_q, kv_lens, slots, positions, admitted = out
@@ -575,7 +576,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         _paged_check(torch.uint8, device, (ws, "workspace", ws.shape))
         if ws.numel() < nb or ws.data_ptr() % 32 != 0:
             raise ValueError(f"workspace must have at least {nb} bytes and begin at a multiple of 32")
-    if made:
+    if made and torch._C._cuda_isCurrentStreamCapturing():
         _paged_own("out= and workspace=", *made)
     _lib.call("std_paged_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
               cu_q.data_ptr(), kv_lens.data_ptr(), T, B, Hq, Hkv, D, 1 if dtype == torch.float16 else 0, num_pages,
