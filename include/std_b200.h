@@ -341,7 +341,8 @@ int std_paged_rope_append(const void* qkv, int T, int Hq, int Hkv, int D, int is
  * that sees no key gives 0 and -inf; rows outside every request are left as
  * they were.  scale > 0; Hq / Hkv a whole number <= 128.  What lies in the
  * cache past a request's keys is not used, whatever it holds; a non-finite V
- * row of a new token may reach the other new tokens of its request.
+ * row of a new token may reach the other new tokens of its request.  A NaN or
+ * +inf score makes its row NaN; a key with a score of -inf counts as not seen.
  * A cu_q or kv_lens entry that does not fit T or max_blocks is reported (error
  * 3), the request skipped or its keys cut; a page id outside the pool is
  * reported (error 2) and read as zeros.

@@ -307,6 +307,7 @@ struct PagedShared {
   };
   float m_sum[2][PA_FEW];  // few rows: m of each stream's sum in global memory
   alignas(16) int flag[2][2][4];  // few rows: a vote per warp, by step parity
+  int open[2];                    // few rows: some row's m is not set yet
   PagedPiece piece[PA_PIECES];
   uint32_t tmem;
 };
@@ -544,8 +545,9 @@ STD_DEV bool paged_softmax_half(uint32_t tS, uint32_t tO, float sc, int nvis, bo
   tmem_wait_st();
   tc_fence_before();
   const float2 l = f2_split(f2_add(l2[0], l2[1]));
-  // A NaN or infinite score makes its row NaN: it has left a NaN here or, through
-  // ex2_fma2, FLT_MAX or more; sums of numbers stay below 2^31 2^PA_RESCALE.
+  // A NaN or +inf score makes its row NaN: it has left a NaN here or, through
+  // ex2_fma2, FLT_MAX or more; sums of numbers stay below 2^31 2^PA_RESCALE.  (-inf has
+  // weight 0, as a hidden key.)
   l_run += l.x + l.y;
   if (!(l_run < 1e30f)) l_run = NAN;
   return true;
@@ -578,9 +580,10 @@ STD_DEV int warp_reduce_rows(float* v, int lane, Op op) {
 // stream's S, O, join and group barriers; bar_q_empty: its query slot's.  False
 // when a wait ran out.  sV: the stage of the piece's last V; ntail: tails cleared.
 //
-// m (sh.ref) is set to the row's maximum over the first block and raised when a
-// score passes it by 2^8, on all four warps: they vote at every block.  The keys
-// a row sees are a prefix, so a row without one in the first block has none.
+// m (sh.ref) is set to the row's maximum over the first block that has one (a
+// visible score above -inf: as a rule the first block) and raised when a score passes
+// it by 2^8, on all four warps: they vote at every block.  Until it is set it is 0, the
+// row's P, l and O are 0, and the vote is taken as given.
 template <typename T, int D, int N, int ST>
 STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, PagedShared<ST>& sh, uint8_t* sQ,
                              uint8_t* sV, uint32_t tS, uint32_t tO, int s, uint64_t* bar_q_empty, uint32_t& ntail,
@@ -611,7 +614,8 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
         float v = __uint_as_float(o[j]);
         if (key < D) {
           float* at = sum + static_cast<size_t>(c + j) * D;
-          if (!begin) v = fmaf(*at, ex2_approx(sh.m_sum[s][c + j] - sh.ref[s][c + j]), v);
+          // (m only rises; set below 0 after the sum began, the sum is 0)
+          if (!begin) v = fmaf(*at, ex2_approx(fminf(sh.m_sum[s][c + j] - sh.ref[s][c + j], 0.f)), v);
           if (!end) *at = v;
         }
         o[j] = end ? __float_as_uint(v) : 0u;
@@ -628,6 +632,7 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
   float l[N];
 #pragma unroll
   for (int n = 0; n < N; ++n) l[n] = 0.f;
+  bool set = false, open = true;  // m of row `key` (key < N); some row's is not set yet
 #pragma unroll 1
   for (int k = 0; k < steps; ++k, ++ns) {
     if (!__all_sync(0xffffffffu, mbar_wait(&sh.bar_s[s][0], ns & 1))) return false;
@@ -649,8 +654,8 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
       y[n + 3] = n + 3 >= hide && n + 3 < rows ? fmaf(y[n + 3], sc, -m.w) : -INFINITY;
       over = fmaxf(max3(over, y[n], y[n + 1]), fmaxf(y[n + 2], y[n + 3]));
     }
-    bool raise = k == 0;
-    if (k > 0) {
+    bool raise = open;
+    if (!open) {
       const bool vote = __any_sync(0xffffffffu, over > PA_RESCALE);
       if (lane == 0) sh.flag[s][k & 1][w] = vote ? 1 : 0;
       if (!group_sync()) return false;
@@ -666,23 +671,28 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
       if (!group_sync()) return false;
       if (key < N) {
         const float mx = fmaxf(fmaxf(red(s, 0, key), red(s, 1, key)), fmaxf(red(s, 2, key), red(s, 3, key)));
-        const float up = k == 0 ? (mx > -INFINITY ? mx : 0.f) : (mx > PA_RESCALE ? mx : 0.f);
+        const float up = set ? (mx > PA_RESCALE ? mx : 0.f) : (mx > -INFINITY ? mx : 0.f);
+        set = set || mx > -INFINITY || key >= rows;
         sh.up[s][key] = up;
         sh.ref[s][key] = k == 0 ? up : sh.ref[s][key] + up;
+        const uint32_t unset = __ballot_sync(N == 32 ? 0xffffffffu : (1u << N) - 1, !set);
+        if (key == 0) sh.open[s] = unset != 0 ? 1 : 0;
       }
       if (!group_sync()) return false;
+      open = sh.open[s] != 0;
 #pragma unroll
       for (int n = 0; n < N; ++n) y[n] -= sh.up[s][n];
       if (k > 0) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) l[n] *= ex2_approx(-sh.up[s][n]);
+        for (int n = 0; n < N; ++n) l[n] *= ex2_approx(-fmaxf(sh.up[s][n], 0.f));  // (below 0: l is 0)
         uint32_t o[16];
 #pragma unroll 1
         for (int c = 0; c < N; c += 16) {
           tmem_ld16(tO + c, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * ex2_approx(-sh.up[s][c + j]));
+          for (int j = 0; j < 16; ++j)
+            o[j] = __float_as_uint(__uint_as_float(o[j]) * ex2_approx(-fmaxf(sh.up[s][c + j], 0.f)));
           tmem_st16(tO + c, o);
         }
         tmem_wait_st();

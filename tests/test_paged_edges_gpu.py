@@ -149,6 +149,99 @@ def test_graphs_of_torch_need_no_workspace(ops):
     _no_device_error(ops)
 
 
+# ------------------------------------------------------------------ scores of -inf
+def far_below(x, lowest):
+    """Every score of x strongly negative, and -inf at the keys `lowest(L)` (a mask)."""
+    x.q = x.q.abs().clamp(0.5, 2)
+    for b in range(len(x.pairs)):
+        keys = (-40 * x.keys[b][0].float().abs().clamp(0.8, 1.2)).to(x.dtype)
+        keys[lowest(x.kv[b])] = -math.inf
+        set_keys(x, b, keys)
+
+
+def check_hidden(x, out, lse, causal):
+    """Paged.check for keys that hold -inf: such a key counts as hidden."""
+    e, at, (Hq, D) = torch.finfo(x.dtype).eps, 0, x.q.shape[1:]
+    G = Hq // x.k.shape[1]
+    for b, (_, n) in enumerate(x.pairs):
+        L = x.kv[b]
+        q = x.q[at:at + n].double().permute(1, 0, 2)
+        k, v = (t.double().permute(1, 0, 2).repeat_interleave(G, 0) for t in x.keys[b])
+        hidden = k.isinf().any(-1)[:, None, :].expand(Hq, n, L)
+        k = torch.where(k.isinf(), 0.0, k)
+        if causal:
+            hidden = hidden | (torch.arange(L, device="cuda")[None] > (L - n + torch.arange(n, device="cuda"))[:, None])
+        s = (q @ k.transpose(1, 2) / math.sqrt(D)).masked_fill(hidden, -math.inf)
+        size = (q.abs() @ k.abs().transpose(1, 2) / math.sqrt(D)).amax(-1, keepdim=True)
+        m = s.amax(-1, keepdim=True)
+        some = m > -math.inf
+        p = torch.exp(s - torch.where(some, m, 0.0))
+        l = torch.where(some, p.sum(-1, keepdim=True), 1.0)
+        ref, A = p @ v / l, p @ v.abs() / l
+        d = D * 2.0 ** -24 * size + 2.0 ** -22 + (34 + L / 64) * 2.0 ** -24
+        tol = 1.01 * (e / 2 * ref.abs() + (e / 2 + 2 * d) * A)
+        if x.dtype == FP:
+            tol = tol + 2.0 ** -25 * (~hidden).double() @ v.abs() / l + 2.0 ** -25
+        got = out[at:at + n].double().permute(1, 0, 2)
+        assert torch.isfinite(got).all() and ((got - ref).abs() <= tol + 1e-30).all(), b
+        want, g2 = torch.where(some, m + l.log(), -math.inf)[..., 0], lse[at:at + n].double().t()
+        assert torch.equal(g2 == -math.inf, want == -math.inf), b
+        fin = want > -math.inf
+        t2 = 2 * d[..., 0] + (2 * want.abs() + 16) * 2.0 ** -22
+        assert ((g2 - want).abs()[fin] <= t2[fin]).all(), b
+        at += n
+
+
+@pytest.mark.parametrize("D,dtype", [(64, FP), (128, BF)])
+@pytest.mark.parametrize("first,count", [(0, 128), (0, 129), (0, 256), (0, 700), (128, 128), (64, 5000), (0, 100000)])
+def test_scores_of_minus_infinity(ops, D, dtype, first, count):
+    """Keys with a score of -inf over whole blocks, a request's first ones or all of them
+    among these, before finite scores far below 0: they count as hidden, in every form
+    (few rows, one tile, a pair, divided over CTAs)."""
+    x = Paged([(300, 1), (290, 4), (290, 15), (200, 100), (1300, 2), (6000, 2), (3000, 30), (255, 1)], 14, 2, D, 64, dtype,
+              seed=count)
+    far_below(x, lambda L: (torch.arange(L, device="cuda") >= first) & (torch.arange(L, device="cuda") < first + count))
+    lse = torch.empty(x.q.shape[:2], device="cuda")
+    for causal in (True, False):
+        out = x.call(ops, causal, lse=lse)
+        check_hidden(x, out, lse, causal)
+    _no_device_error(ops)
+
+
+@pytest.mark.parametrize("new,D,dtype", [(1, 64, FP), (4, 128, BF), (12, 64, BF), (36, 128, FP)])
+def test_scores_of_minus_infinity_past_the_long_sums(ops, new, D, dtype):
+    """150 requests of 2^18 keys on the same pages, the first 153,600 keys with a score of
+    -inf: a CTA's sums are put aside (after 2^17 keys at the latest) before any score counts."""
+    L, page, G, B, start = 1 << 18, 256, 7, 150, 600
+    g = torch.Generator(device="cuda").manual_seed(new)
+    k = -40 * torch.randn(3, 1, page, D, generator=g, device="cuda").abs().clamp(0.8, 1.2)
+    k[0, ..., 0] = -math.inf
+    k = k.to(dtype)
+    v = (torch.rand(3, 1, page, D, generator=g, device="cuda") + 0.5).to(dtype)
+    ids = torch.arange(L // page, device="cuda")
+    row = torch.where(ids < start, 0, 1 + ids % 2).int()
+    q = torch.randn(B * new, G, D, generator=g, device="cuda").abs().clamp(0.5, 2).to(dtype)
+    lse = torch.empty(B * new, G, device="cuda")
+    cu, kv = torch.arange(0, B * new + 1, new, device="cuda").int(), torch.full((B,), L, device="cuda").int()
+    out = ops.paged_attention(q, k, v, row.expand(B, -1).contiguous(), cu, kv, causal=False, lse=lse).double()
+    s = torch.einsum("nhd,pkd->nhpk", q.double(), k[1:, 0].double()) / math.sqrt(D)
+    size = torch.einsum("nhd,pkd->nhpk", q.double(), k[1:, 0].double().abs()).amax((-1, -2)) / math.sqrt(D)
+    m = s.amax((-1, -2), keepdim=True)
+    w = torch.exp(s - m) * ((L // page - start) / 2)
+    l = w.sum((-1, -2))
+    ref = torch.einsum("nhpk,pkd->nhd", w, v[1:, 0].double()) / l[..., None]
+    e = torch.finfo(dtype).eps
+    # output and probabilities rounded once each (v > 0: A = ref), scores as sums of D products, and sums of at
+    # most 2^18 / 16 additions that are cut off (2^-23 of the sum each) in the products, 2^18 / 256 in l
+    d = 2 * (D * 2.0 ** -24 * size + 2.0 ** -22)
+    low = 2.0 ** -25 * (L - start * page) * v.max().double() / l if dtype == FP else torch.zeros_like(l)
+    tol = (e + (2 ** 13 + 2 ** 9) * 2.0 ** -23 + d[..., None]) * ref + low[..., None]
+    assert ((out - ref).abs() <= 1.01 * tol).all(), ((out - ref).abs() / tol).max().item()
+    want = l.log() + m[..., 0, 0]
+    assert ((lse.double() - want).abs() <= d + 2.0 ** 9 * 2.0 ** -23 + (2 * want.abs() + 16) * 2.0 ** -22).all()
+    _no_device_error(ops)
+
+
 # ------------------------------------------------------------------ idle requests
 @pytest.mark.parametrize("B", [33, 64, 2047, 8192])
 def test_mostly_idle_batches(ops, B):
