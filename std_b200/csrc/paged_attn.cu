@@ -69,6 +69,12 @@ constexpr int PA_CTAS = 148;     // one CTA per SM
 constexpr int PA_THREADS = 384;  // 2 softmax warpgroups; TMA, two MMA and a scheduler warp
 constexpr int PA_BN = 128;       // keys per block
 constexpr float PA_RESCALE = 8.0f;  // log2 units
+// log2 of the largest P when m is set: P lies between 2^-24 (a half's smallest
+// number) and 2^(top + PA_RESCALE) at most, below a half's 65504.  Weights under 2^(-25 - top) of the
+// largest are lost, which many keys of small weight beside a heavy one notice (2^17
+// keys of 2^-25 each: 0.4 % of the row with top 0).  bf16 has the range of a float.
+template <typename T>
+constexpr float PA_TOP = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 // Cost of a block in a single and in a pair (measured: 2000 to 2400 cycles and
 // 3200 to 3700); an item costs PA_OVER blocks more (its queries, first keys and output).
 constexpr int PA_W1 = 3, PA_W2 = 5, PA_OVER = 3;
@@ -502,11 +508,11 @@ STD_DEV bool paged_softmax_half(uint32_t tS, uint32_t tO, float sc, int nvis, bo
 #pragma unroll
     for (int c = 0; c < 4; ++c) m4[c] = max3(m4[c], __uint_as_float(x[j + c]), __uint_as_float(x[j + 4 + c]));
   const float m_c = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;  // scale > 0
-  const bool need = m_run != -INFINITY && m_c > m_run + PA_RESCALE;
+  const bool need = m_run != -INFINITY && m_c > m_run + (PA_RESCALE + PA_TOP<T>);
   if (__any_sync(0xffffffffu, need)) {
     if (!__all_sync(0xffffffffu, mbar_wait(bar_next, next & 1))) return false;  // O at rest
     tc_fence_after();
-    const float alpha = need ? exp2f(m_run - m_c) : 1.0f;
+    const float alpha = need ? exp2f(m_run - (m_c - PA_TOP<T>)) : 1.0f;
     uint32_t o[32];
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
@@ -518,10 +524,10 @@ STD_DEV bool paged_softmax_half(uint32_t tS, uint32_t tO, float sc, int nvis, bo
     }
     if (need) {
       l_run *= alpha;
-      m_run = m_c;
+      m_run = m_c - PA_TOP<T>;
     }
   }
-  if (m_run == -INFINITY) m_run = m_c;
+  if (m_run == -INFINITY) m_run = m_c - PA_TOP<T>;
   // a row that has seen no key yet keeps P = 2^-inf = 0
   const float nm = m_run == -INFINITY ? 0.f : -m_run;
   const uint64_t sc2 = f2_make(sc, sc), nm2 = f2_make(nm, nm);
@@ -546,7 +552,7 @@ STD_DEV bool paged_softmax_half(uint32_t tS, uint32_t tO, float sc, int nvis, bo
   tc_fence_before();
   const float2 l = f2_split(f2_add(l2[0], l2[1]));
   // A NaN or +inf score makes its row NaN: it has left a NaN here or, through
-  // ex2_fma2, FLT_MAX or more; sums of numbers stay below 2^31 2^PA_RESCALE.  (-inf has
+  // ex2_fma2, FLT_MAX or more; sums of numbers stay below 2^31 2^(PA_RESCALE + 7).  (-inf has
   // weight 0, as a hidden key.)
   l_run += l.x + l.y;
   if (!(l_run < 1e30f)) l_run = NAN;
@@ -656,7 +662,7 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
     }
     bool raise = open;
     if (!open) {
-      const bool vote = __any_sync(0xffffffffu, over > PA_RESCALE);
+      const bool vote = __any_sync(0xffffffffu, over > PA_RESCALE + PA_TOP<T>);
       if (lane == 0) sh.flag[s][k & 1][w] = vote ? 1 : 0;
       if (!group_sync()) return false;
       const int4 f = *reinterpret_cast<const int4*>(sh.flag[s][k & 1]);
@@ -671,7 +677,7 @@ STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, 
       if (!group_sync()) return false;
       if (key < N) {
         const float mx = fmaxf(fmaxf(red(s, 0, key), red(s, 1, key)), fmaxf(red(s, 2, key), red(s, 3, key)));
-        const float up = set ? (mx > PA_RESCALE ? mx : 0.f) : (mx > -INFINITY ? mx : 0.f);
+        const float up = mx > (set ? PA_RESCALE + PA_TOP<T> : -INFINITY) ? mx - PA_TOP<T> : 0.f;
         set = set || mx > -INFINITY || key >= rows;
         sh.up[s][key] = up;
         sh.ref[s][key] = k == 0 ? up : sh.ref[s][key] + up;

@@ -242,6 +242,50 @@ def test_scores_of_minus_infinity_past_the_long_sums(ops, new, D, dtype):
     _no_device_error(ops)
 
 
+@pytest.mark.parametrize("new,D,dtype", [(1, 64, FP), (4, 128, FP), (12, 64, FP), (36, 64, FP), (1, 64, BF), (36, 128, BF)])
+@pytest.mark.parametrize("below", [19.3, 25.3])
+def test_many_small_weights_beside_a_large_one(ops, new, D, dtype, below):
+    """A first key that holds nearly all of a row and 2^17 others of 2^-below of its weight
+    each, in one CTA (150 requests on the same pages).
+
+    Half precision rounds such a probability to a multiple of 2^-24 of the kernel's unit,
+    in which the largest is at least 2^7: off by at most 2^-32 of the largest weight.
+    bf16 has the usual e / 2.  The sums: at most 2^17 / 16 additions that are cut off,
+    2^-23 of the sum each."""
+    L, page, G, B = 1 << 17, 256, 7, 150
+    g = torch.Generator(device="cuda").manual_seed(new)
+    k = torch.zeros(3, 1, page, D, device="cuda")
+    k[..., 1] = 0.2 * torch.rand(3, 1, page, generator=g, device="cuda")
+    k[0, 0, 0, 0] = below * math.log(2) * math.sqrt(D) / 4
+    k = k.to(dtype)
+    v = (torch.rand(3, 1, page, D, generator=g, device="cuda") + 0.5).to(dtype)
+    v[0, 0, 0] = 0
+    row = torch.arange(L // page, device="cuda").int() % 2 + 1
+    row[0] = 0
+    q = torch.zeros(B * new, G, D, device="cuda")
+    q[..., 0] = 4
+    q[..., 1] = torch.rand(B * new, G, generator=g, device="cuda")
+    q = q.to(dtype)
+    lse = torch.empty(B * new, G, device="cuda")
+    cu, kv = torch.arange(0, B * new + 1, new, device="cuda").int(), torch.full((B,), L, device="cuda").int()
+    out = ops.paged_attention(q, k, v, row.expand(B, -1).contiguous(), cu, kv, causal=False, lse=lse).double()
+    count = torch.stack([(row == i).sum() for i in range(3)]).double()[:, None]
+    s = torch.einsum("nhd,pkd->nhpk", q.double(), k[:, 0].double()) / math.sqrt(D)
+    m = s.amax((-1, -2), keepdim=True)
+    w = torch.exp(s - m) * count
+    l = w.sum((-1, -2))
+    ref = torch.einsum("nhpk,pkd->nhd", w, v[:, 0].double()) / l[..., None]
+    e = torch.finfo(dtype).eps
+    d = 2 * (D * 2.0 ** -24 * m[..., 0, 0].abs() + 2.0 ** -22)[..., None]
+    tol = (e + 2.0 ** 13 * 2.0 ** -23 + d) * ref  # (v >= 0: the output's and the probabilities' e / 2)
+    if dtype == FP:
+        tol = tol + 2.0 ** -32 * L * v.max().double() + 2.0 ** -25
+    assert ((out - ref).abs() <= 1.01 * tol).all(), ((out - ref).abs() / tol).max().item()
+    want = l.log() + m[..., 0, 0]
+    assert ((lse.double() - want).abs() <= d[..., 0] + 2.0 ** 9 * 2.0 ** -23 + (2 * want.abs() + 16) * 2.0 ** -22).all()
+    _no_device_error(ops)
+
+
 # ------------------------------------------------------------------ idle requests
 @pytest.mark.parametrize("B", [33, 64, 2047, 8192])
 def test_mostly_idle_batches(ops, B):
