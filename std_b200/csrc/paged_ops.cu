@@ -149,8 +149,10 @@ __global__ void __launch_bounds__(1024) paged_update_kernel(const PagedUpdatePar
     if (run[0] > (p.max_tokens > 0 ? p.max_tokens : 0x7fffffffll)) std_set_error(STD_DEVERR_LENGTH);
     if (static_cast<long long>(n_free) + back > p.num_pages) std_set_error(STD_DEVERR_BOUNDS);
   }
-  // returns: page r of the whole step, ids cleared from the table
-  for (int r = tid; r < back; r += nt) {
+  // returns: page r of the whole step, ids cleared from the table (unsigned: `back` may
+  // come near 2^31 where n_blocks claims more pages than there are)
+  for (uint32_t u = tid; u < static_cast<uint32_t>(back); u += nt) {
+    const int r = static_cast<int>(u);
     const int b = paged_owner(s_back, p.B, r);
     const int total = (b + 1 < p.B ? s_back[b + 1] : back) - s_back[b];
     int32_t* at = p.table + static_cast<size_t>(b) * p.width + (p.n_blocks[b] - total + (r - s_back[b]));
@@ -375,7 +377,7 @@ extern "C" int std_paged_update(const int32_t* past_lens, const int32_t* new_len
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (launch_pdl(stdb::paged_update_kernel, dim3(1), dim3(threads), smem, s, p) != cudaSuccess) return 4;
   if (!p.tokens_here &&
-      launch_pdl(stdb::paged_tokens_kernel, dim3((max_tokens + 255) / 256), dim3(256), 0, s, p) != cudaSuccess)
+      launch_pdl(stdb::paged_tokens_kernel, dim3((max_tokens - 1) / 256 + 1), dim3(256), 0, s, p) != cudaSuccess)
     return 4;
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }

@@ -326,3 +326,18 @@ def test_idle_requests_are_passed_quickly(ops):
         x.check(out, None)
     assert times[1] < 3 * times[0], times
     _no_device_error(ops)
+
+
+# ------------------------------------------------------------------ tables
+@pytest.mark.parametrize("max_tokens", [2 ** 31 - 256, 2 ** 31 - 1])
+def test_update_with_the_most_tokens(ops, max_tokens):
+    """Slots and positions for as many tokens as 32 bits count."""
+    table, held = torch.full((2, 8), -1, dtype=torch.int32, device="cuda"), _i32([0, 0])
+    free, n_free = torch.arange(8, dtype=torch.int32, device="cuda"), _i32([8])
+    cu, kv, slots, pos, ok = ops.paged_update(_i32([3, 0]), _i32([20, 3]), table, held, free, n_free, 16, max_tokens)
+    assert cu.tolist() == [0, 20, 23] and kv.tolist() == [23, 3] and ok.tolist() == [1, 1]
+    assert slots[:23].tolist() == [7 * 16 + i for i in range(3, 16)] + [6 * 16 + i for i in range(7)] + [80, 81, 82]
+    assert pos[:23].tolist() == list(range(3, 23)) + [0, 1, 2]
+    assert slots.numel() == max_tokens and slots[23:].amax() == -1 and pos[23:].amax() == -1
+    assert slots[23:].amin() == -1 and pos[23:].amin() == -1
+    _no_device_error(ops)
