@@ -459,8 +459,11 @@ def paged_update(past_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
     if block_table.dim() != 2:
         raise ValueError("block_table must be [B, max_blocks]")
     width, num_pages, max_tokens = block_table.shape[1], free_pages.numel(), int(max_tokens)
+    page_size = int(page_size)
     if not 0 <= max_tokens < 2 ** 31:
         raise ValueError("max_tokens must be a non-negative int32")
+    if not (0 <= page_size < 2 ** 31 and width < 2 ** 31 and num_pages < 2 ** 31):  # (ctypes would cut them)
+        raise ValueError(f"page_size, max_blocks and num_pages must be int32, got {page_size}, {width} and {num_pages}")
     _paged_check(i32, device, (past_lens, "past_lens", (B,)), (new_lens, "new_lens", (B,)),
                  (block_table, "block_table", (B, width)), (n_blocks, "n_blocks", (B,)),
                  (free_pages, "free_pages", (num_pages,)), (n_free, "n_free", (1,)))
@@ -476,7 +479,7 @@ def paged_update(past_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
                      (slots, "slots", (max_tokens,)), (positions, "positions", (max_tokens,)),
                      (admitted, "admitted", (B,)))
     _lib.call("std_paged_update", past_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
-              n_blocks.data_ptr(), free_pages.data_ptr(), n_free.data_ptr(), B, width, int(page_size), num_pages,
+              n_blocks.data_ptr(), free_pages.data_ptr(), n_free.data_ptr(), B, width, page_size, num_pages,
               max_tokens, cu_q.data_ptr(), kv_lens.data_ptr(), slots.data_ptr(), positions.data_ptr(),
               admitted.data_ptr(), _stream_of(device))
     return cu_q, kv_lens, slots, positions, admitted
@@ -553,6 +556,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError(f"query heads ({Hq}) must be a multiple of key heads ({Hkv}), at most 128 times as many")
     _paged_check(torch.int32, device, (block_table, "block_table", (B, width)), (cu_q, "cu_q", (B + 1,)),
                  (kv_lens, "kv_lens", (B,)))
+    if width >= 2 ** 31:
+        raise ValueError(f"block_table has {width} entries a request, more than int32 counts")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 0.0 < scale < 3e38:
         raise ValueError(f"scale must be positive and finite, got {scale}")

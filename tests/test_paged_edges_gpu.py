@@ -341,3 +341,19 @@ def test_update_with_the_most_tokens(ops, max_tokens):
     assert slots.numel() == max_tokens and slots[23:].amax() == -1 and pos[23:].amax() == -1
     assert slots[23:].amin() == -1 and pos[23:].amin() == -1
     _no_device_error(ops)
+
+
+def test_sizes_beyond_32_bits_are_refused(ops):
+    """Sizes that differ from served ones by 2^32."""
+    i = _i32([0])
+    wide = torch.empty(1, 2 ** 32 + 8, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="page_size"):
+        ops.paged_update(i, i, _i32([[-1] * 8]), i, i, i, 2 ** 32 + 16, 4)
+    with pytest.raises(ValueError, match="max_blocks"):
+        ops.paged_update(i, i, wide, i, i, i, 16, 4)
+    with pytest.raises(ValueError, match="num_pages"):
+        ops.paged_update(i, i, _i32([[-1] * 8]), i, wide.view(-1), i, 16, 4)
+    x = Paged([(30, 2)], 28, 4, 128, 16, BF)
+    with pytest.raises(ValueError, match="int32"):
+        ops.paged_attention(x.q, x.k, x.v, wide, x.cu, x.kv_lens)
+    _no_device_error(ops)
