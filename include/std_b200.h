@@ -339,7 +339,7 @@ int std_paged_rope_append(const void* qkv, int T, int Hq, int Hkv, int D, int is
  * n new ones last; causal: token t sees keys 0 .. kv_len - n + t, else all
  * kv_len.  out [T, Hq, D]; lse [T, Hq] fp32 natural log (may be NULL).  A row
  * that sees no key gives 0 and -inf; rows outside every request are left as
- * they were.  scale > 0; Hq / Hkv a whole number <= 128.  What lies in the
+ * they were.  0 < scale < 2.3e38; Hq / Hkv a whole number <= 128.  What lies in the
  * cache past a request's keys is not used, whatever it holds; a non-finite V
  * row of a new token may reach the other new tokens of its request.  A NaN or
  * +inf score makes its row NaN; a key with a score of -inf counts as not seen.

@@ -1626,7 +1626,7 @@ extern "C" int std_paged_attn(const void* q, const void* k_pages, const void* v_
   if ((D != 64 && D != 128) || T < 0 || B <= 0 || B > STD_PAGED_MAX_REQUESTS || Hkv <= 0 || Hkv > 65535 || Hq <= 0 ||
       Hq % Hkv != 0 || Hq / Hkv > 128 || num_pages <= 0 || max_blocks <= 0 || !paged_page_ok(page_size))
     return 1;
-  if (!(scale > 0.f) || !(scale < 3.4e38f)) return 1;
+  if (!(scale > 0.f) || !(scale * 1.4426950408889634f < 3.4e38f)) return 1;
   // int32 indexes: keys of a request, slots, 8-row groups of the pool (one page more: the zero fill)
   if (static_cast<long long>(max_blocks) * page_size > 0x7fffffffll - 1024 ||
       static_cast<long long>(num_pages) * page_size > 0x7fffffffll ||

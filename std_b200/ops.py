@@ -559,8 +559,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if width >= 2 ** 31:
         raise ValueError(f"block_table has {width} entries a request, more than int32 counts")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 0.0 < scale < 3e38:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not 0.0 < scale < 2.3e38:  # (times log2 e it has to be a float)
+        raise ValueError(f"scale must be positive and below 2.3e38, got {scale}")
     made = ()  # here
     if out is None:
         out = torch.empty_like(q)

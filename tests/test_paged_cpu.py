@@ -86,3 +86,8 @@ def test_wrappers_refuse_cpu_tensors():
         ops.paged_update(i, i, i.view(2, 1), i, i, i[:1], 16, 4)
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.paged_rope_append(q.view(2, 64), i, i, k[0, 0], k[0, 0], q, k, k)
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3e38, 3.3e38])
+def test_attention_refuses_scales_that_overflow_in_log2(scale):
+    assert attn(scale=scale) == 1
