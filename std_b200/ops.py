@@ -384,6 +384,7 @@ def argmax_rows(logits: torch.Tensor, out: torch.Tensor, n: int = 1, out_stride:
 # ----------------------------------------------------------------------------
 
 _PAGED_DTYPES = (torch.bfloat16, torch.float16)
+_PAGED_SIZES = (16, 32, 64, 128, 256)
 _PAGED_WS_BYTES: Dict[int, int] = {}
 
 
@@ -431,7 +432,7 @@ def _paged_pool(k_pages: torch.Tensor, v_pages: torch.Tensor, dtype: torch.dtype
         raise ValueError("k_pages must be [num_pages, Hkv, page_size, D]")
     shape = k_pages.shape
     _paged_check(dtype, device, (k_pages, "k_pages", shape), (v_pages, "v_pages", shape))
-    if shape[2] not in (16, 32, 64, 128, 256):
+    if shape[2] not in _PAGED_SIZES:
         raise ValueError(f"page_size must be 16, 32, 64, 128 or 256, got {shape[2]}")
     if shape[3] not in (64, 128):
         raise ValueError(f"head dim must be 64 or 128, got {shape[3]}")
@@ -449,13 +450,12 @@ def paged_update(past_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
     taken from or returned to the end of the free list, so new_lens 0 with a
     shorter past_lens rolls a request back.  Returns (cu_q [B + 1], kv_lens [B],
     slots [max_tokens], positions [max_tokens], admitted [B]); a request that the
-    list cannot serve has admitted 0, kv_lens 0 and slots -1.  `out` gives the
+    list cannot serve has admitted 0, kv_lens 0 and slots -1.  A step without
+    requests (B 0) gives cu_q [0] and slots of -1.  `out` gives the
     five result tensors (a captured graph's static buffers; the captured body of a
     loop or branch needs it)."""
     device = _paged_device(past_lens, "past_lens")
     B, i32 = past_lens.numel(), torch.int32
-    if B < 1:
-        raise ValueError("paged_update needs at least one request")
     if block_table.dim() != 2:
         raise ValueError("block_table must be [B, max_blocks]")
     width, num_pages, max_tokens = block_table.shape[1], free_pages.numel(), int(max_tokens)
@@ -478,6 +478,13 @@ def paged_update(past_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
         _paged_check(i32, device, (cu_q, "cu_q", (B + 1,)), (kv_lens, "kv_lens", (B,)),
                      (slots, "slots", (max_tokens,)), (positions, "positions", (max_tokens,)),
                      (admitted, "admitted", (B,)))
+    if B == 0:  # nothing to do but to say so
+        if page_size not in _PAGED_SIZES:
+            raise ValueError(f"page_size must be 16, 32, 64, 128 or 256, got {page_size}")
+        cu_q.zero_()
+        slots.fill_(-1)
+        positions.fill_(-1)
+        return cu_q, kv_lens, slots, positions, admitted
     _lib.call("std_paged_update", past_lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(),
               n_blocks.data_ptr(), free_pages.data_ptr(), n_free.data_ptr(), B, width, page_size, num_pages,
               max_tokens, cu_q.data_ptr(), kv_lens.data_ptr(), slots.data_ptr(), positions.data_ptr(),
@@ -538,7 +545,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     kv_len - n + t (causal) or all kv_len.  bf16 or fp16; any Hq / Hkv up to 128.
     scale defaults to 1 / sqrt(D).  out [T, Hq, D], lse [T, Hq] fp32 (optional).
     Rows that see no key give 0 and -inf; rows outside every request are left
-    as they were (uninitialised in an `out` made here).  workspace (optional): a
+    as they were (uninitialised in an `out` made here): all of them in a step
+    without requests.  workspace (optional): a
     buffer of paged_attention_workspace, which no other call may use before this
     one has run; one kept by the caller serves a whole sequence of calls.  The
     captured body of a loop or branch needs `out` and `workspace`."""
@@ -583,6 +591,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
             raise ValueError(f"workspace must have at least {nb} bytes and begin at a multiple of 32")
     if made and torch._C._cuda_isCurrentStreamCapturing():
         _paged_own("out= and workspace=", *made)
+    if B == 0:  # every row is outside every request
+        return out
     _lib.call("std_paged_attn", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(),
               cu_q.data_ptr(), kv_lens.data_ptr(), T, B, Hq, Hkv, D, 1 if dtype == torch.float16 else 0, num_pages,
               page, width, 1 if causal else 0, scale, out.data_ptr(), _p(lse), ws.data_ptr(), nb, _stream_of(device))

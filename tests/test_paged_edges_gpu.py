@@ -357,3 +357,39 @@ def test_sizes_beyond_32_bits_are_refused(ops):
     with pytest.raises(ValueError, match="int32"):
         ops.paged_attention(x.q, x.k, x.v, wide, x.cu, x.kv_lens)
     _no_device_error(ops)
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_steps_without_requests(ops, graph):
+    """A server between requests: the three calls of a step with none, with rows for tokens
+    and without."""
+    cos = torch.ones(4, 64, dtype=BF, device="cuda")
+    k = torch.full((5, 4, 16, 128), 3.0, dtype=BF, device="cuda")
+    v = k.clone()
+    for rows in (0, 6):
+        qkv = torch.zeros(rows, 36 * 128, dtype=BF, device="cuda")
+        q, out = (torch.full((rows, 28, 128), x, dtype=BF, device="cuda") for x in (4.0, 5.0))
+        table, free, n_free = torch.empty(0, 7, dtype=torch.int32, device="cuda"), torch.arange(5, device="cuda").int(), _i32([5])
+        none = _i32([])
+        res = [torch.full((n,), 9, dtype=torch.int32, device="cuda") for n in (1, 0, rows, rows, 0)]
+
+        def step(res):
+            cu, kv, slots, pos, ok = ops.paged_update(none, none, table, none, free, n_free, 16, rows, out=res)
+            ops.paged_rope_append(qkv, pos, slots, cos, cos, q, k, v)
+            ops.paged_attention(q, k, v, table, cu, kv, out=out)
+            return cu, kv, slots, pos, ok
+
+        if graph:
+            g = torch.cuda.CUDAGraph()
+            torch.cuda.synchronize()
+            with torch.cuda.graph(g):
+                got = step(res)
+            g.replay()
+        else:
+            got = step(None)
+        assert [t.tolist() for t in got] == [[0], [], [-1] * rows, [-1] * rows, []]
+        assert (q == 4).all() and (out == 5).all() and (k == 3).all() and (v == 3).all() and n_free.item() == 5
+        assert ops.paged_attention(q, k, v, table, got[0], none).shape == q.shape
+    with pytest.raises(ValueError, match="page_size"):
+        ops.paged_update(none, none, table, none, free, n_free, 24, 0)
+    _no_device_error(ops)
