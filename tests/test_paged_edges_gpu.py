@@ -393,3 +393,50 @@ def test_steps_without_requests(ops, graph):
     with pytest.raises(ValueError, match="page_size"):
         ops.paged_update(none, none, table, none, free, n_free, 24, 0)
     _no_device_error(ops)
+
+
+# ------------------------------------------------------------------ long prompts
+def test_long_prompt_every_row_against_64_bits(ops):
+    """A 40,000-token prompt at once and in odd chunks: every row within its own rounding of
+    the 64-bit value, e / 2 (|o| + A) with A = sum p |v| of that row.  The bound is sharp:
+    each item (36 tokens of a key head's group) would miss it if its rows were zeros or
+    those of the item before."""
+    Hq, Hkv, D, page, n, item = 14, 2, 128, 128, 40000, 36
+    G, e = Hq // Hkv, torch.finfo(BF).eps
+    g = torch.Generator(device="cuda").manual_seed(2)
+    blocks = -(-n // page)
+    q = torch.randn(n, Hq, D, generator=g, device="cuda").to(BF)
+    k = torch.randn(blocks, Hkv, page, D, generator=g, device="cuda").to(BF)
+    v = torch.randn(blocks, Hkv, page, D, generator=g, device="cuda").to(BF)
+    table = torch.randperm(blocks, generator=g, device="cuda").int().view(1, -1)
+    whole = ops.paged_attention(q, k, v, table, _i32([0, n]), _i32([n]))
+    parts, at = torch.empty_like(whole), 0
+    for size in (1, 17, 5000, 13001, 36, 21944, 1):
+        ops.paged_attention(q[at:at + size], k, v, table, _i32([0, size]), _i32([at + size]), out=parts[at:at + size])
+        at += size
+    assert at == n
+    kk, vv = (t[table[0].long()].permute(1, 0, 2, 3).reshape(Hkv, -1, D)[:, :n].double() for t in (k, v))
+    far = kk.norm(dim=-1).amax()
+    before = None
+    for a in range(0, n, 7 * item):
+        b = min(n, a + 7 * item)
+        hidden = torch.arange(b, device="cuda")[None] > torch.arange(a, b, device="cuda")[:, None]
+        for h in range(Hkv):
+            rows = q[a:b, h * G:(h + 1) * G].double()
+            p = torch.einsum("thd,ld->htl", rows, kk[h, :b]).div_(math.sqrt(D)).masked_fill_(hidden, -math.inf)
+            p = torch.softmax(p, -1)
+            ref, A = torch.einsum("htl,ld->thd", p, vv[h, :b]), torch.einsum("htl,ld->thd", p, vv[h, :b].abs())
+            del p
+            # scores: sums of D products, |q| |k| at most; sums of n probabilities, 16 at a time and cut off (2^-23)
+            d = D * 2.0 ** -24 * rows.norm(dim=-1, keepdim=True) * far / math.sqrt(D) + 2.0 ** -22 + (34 + n / 8) * 2.0 ** -24
+            tol = 1.01 * (e / 2 * ref.abs() + (e / 2 + 2 * d) * A)
+            for out in (whole, parts):
+                off = (out[a:b, h * G:(h + 1) * G].double() - ref).abs()
+                assert (off <= tol).all(), (a, h, (off / tol).max().item())
+            others = torch.cat([ref[:item] if before is None else before, ref])[:b - a]
+            before = ref[-item:] if h == Hkv - 1 else before
+            for i in range(0, b - a, item):
+                assert (ref[i:i + item].abs() > tol[i:i + item]).any(), (a, i, h)
+                if a + i > 0:
+                    assert ((others[i:i + item] - ref[i:i + item]).abs() > tol[i:i + item]).any(), (a, i, h)
+    _no_device_error(ops)
