@@ -291,8 +291,8 @@ int std_collect_relevance(const void* q, const void* k_cache, const int32_t* vis
  * position x lies in page block_table[b][x / page_size] (block_table [B,
  * max_blocks] int32), row x % page_size; its slot is page * page_size + row.
  * B <= STD_PAGED_MAX_REQUESTS; num_pages * page_size, max_blocks * page_size
- * and B * max_blocks fit int32.  No reference counterpart (the reference's
- * caches are contiguous). */
+ * and B * max_blocks fit int32 (std_paged_attn's own limits stand with it).
+ * No reference counterpart (the reference's caches are contiguous). */
 #define STD_PAGED_MAX_REQUESTS 8192
 
 /* One step's tables, from the requests' lengths (all arrays on the device).
@@ -349,7 +349,10 @@ int std_paged_rope_append(const void* qkv, int T, int Hq, int Hkv, int D, int is
  * Same inputs, same bits; a request's last bits may depend on the batch it is
  * in (std_verify_attn's do not).  out and lse overlap no input.  The workspace
  * (std_paged_attn_workspace_bytes, 32-byte aligned) is that of one call at a
- * time. */
+ * time.
+ * Limits beside the section's (status 1): T < 2^30, max_blocks * page_size <=
+ * 2^31 - 1025, (num_pages + 1) * Hkv * page_size / 8 < 2^31, and at most 5e8 items:
+ * (T / (2 * floor(128 * Hkv / Hq)) + B) * Hkv. */
 size_t std_paged_attn_workspace_bytes(int D);
 int std_paged_attn(const void* q, const void* k_pages, const void* v_pages, const int32_t* block_table,
                    const int32_t* cu_q, const int32_t* kv_lens, int T, int B, int Hq, int Hkv, int D, int is_fp16,

@@ -46,19 +46,22 @@
 //
 // What bounds it, and what was measured (B200, replayed from a graph; bf16, 28
 // query heads on 4 key heads, D 128 unless said).  Long prompts: the softmax warps
-// and power; a 2048-token chunk over 31K keys 830 us = 1130 TFLOP/s (0.82 of what
-// cuBLAS sustains under the power cap; 3200 cycles a block of a pair, of which a
-// softmax warp works 2900 and the MMAs need 2560; the clock falls to 1.45 GHz, and
-// in a long run to 1.3: 918 us), an 8192-token prompt 505 us.  S in halves costs 1.5 x
-// the shared-memory reads of N=128 but keeps a half of S ready while the other is
-// multiplied: 866 us with one S of 128 columns a step from one issuing thread, 815
-// with halves and a thread per stream (at the same clock).
+// and power; a 2048-token chunk over 31K keys 825 us = 1130 TFLOP/s in a short run
+// (0.69 of cuBLAS's burst; 3200 cycles a block of a pair, of which a softmax warp
+// works 2900 and the MMAs need 2560; 1.45 GHz) and 945 us = 990 TFLOP/s in a long one
+// (0.72 of what cuBLAS sustains under the power cap; 1.3 GHz), an 8192-token prompt
+// 508 and 528 us.  S in halves costs 1.5 x the shared-memory reads of N=128 but keeps
+// a half of S ready while the other is multiplied: 866 us with one S of 128 columns a
+// step from one issuing thread, 815 with halves and a thread per stream (at the same
+// clock, before the sums of O were divided).
 // Decoding: HBM; 64 requests of 100 to 8000 keys 85 us = 5.7 TB/s (0.88 of the
 // measured copy), one request of 131K keys 50 us = 5.4 TB/s, 8 verify blocks of
-// 10 tokens over 33K keys 100 us = 5.4 TB/s; untransposed, the first two took 118
-// and 67 us, bound by one warp's softmax of 128 columns for 7 live rows.  Short
-// contexts: latency, 7.5 us for one token and 200 keys, half of it finding the
-// share (2 us) and the first page, key and score (2 us).
+// 10 tokens over 33K keys 102 us = 5.3 TB/s (111 in a long run); untransposed, the
+// first two took 118 and 67 us, bound by one warp's softmax of 128 columns for 7 live
+// rows.  Short contexts: latency, one token and 200 keys 7.6 us with a table for up to
+// 512 keys and 8.8 with a wider one, whose call has the merge behind it (half of it
+// finding the share, 2 us, and the first page, key and score, 2 us); 8 single tokens
+// over 1025 keys 15.0 us whatever the table's width.
 #include "common.cuh"
 
 #include <type_traits>
@@ -80,8 +83,8 @@ constexpr float PA_TOP = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 constexpr int PA_W1 = 3, PA_W2 = 5, PA_OVER = 3;
 // An item of at most this many blocks is not divided but goes where it begins: a cut
 // would cost a partial and the merge (2 us) to save at most two blocks (2 us), and
-// calls whose tables allow no longer item need no merge launch (9.6 -> 7.7 us for
-// one token and 200 keys).
+// calls whose tables allow no longer item (up to 512 keys) need no merge launch: one
+// token and 200 keys 7.6 us, 8.8 with a table of 2048 pages of 16.
 constexpr int PA_WHOLE = 4;
 
 // Shared memory: two query slots and a ring of K/V blocks.  A slot holds a
@@ -484,7 +487,7 @@ __device__ __noinline__ void paged_flush(uint32_t tO, float* sum, float f, bool 
 
 // Half a step of a whole tile's softmax: 64 columns of S to P, with the row's
 // running m and l.  nvis: visible columns; cut: some row of the warp has fewer than
-// all (known without a vote: 521 -> 515 us for an 8192-token prompt).  bar_next: the
+// all (known without a vote, which cost 1 % of an 8192-token prompt).  bar_next: the
 // barrier (phase parity `next`) after which the stream's products issued so far are
 // complete.  False when a wait ran out.
 template <typename T, int D>
@@ -1433,11 +1436,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 // Joins the pieces of the items that cuts divide: blocks x work at the item that
 // CTA x's share ends inside, so an item of many pieces has many blocks.  out =
 // sum_c w_c o_c / sum_c w_c l_c with w_c = exp2(m_c - max m), in a fixed order of
-// the pieces.  Latency is what counts (a few loads per row, mostly from L2): the
-// grid is one wave, since each wave of blocks costs a memory round trip even where
-// there is nothing to join, and the loads of two rows by two pieces a warp are in
-// flight together, or, for an item of many pieces (a long context), a row's pieces
-// over eight warps.
+// the pieces.  Latency is what counts (a few loads per row, mostly from L2): each
+// wave of blocks costs a memory round trip even where there is nothing to join, so
+// the grid is one wave (two blocks an item) while no item can be a pair, and two waves
+// (four blocks) where one can, whose rows repay it: two blocks against four, mixed
+// step 56.3 / 54.9 us, 16 heads of D 64 32.5 / 30.8, 8 verify blocks over 33K keys
+// 103.0 / 102.0.  The loads of two rows by two pieces a warp are in flight together, or, for
+// an item of many pieces (a long context), a row's pieces over eight warps.
 constexpr int PM_THREADS = 512;  // (two blocks per SM)
 template <int D>
 struct PagedSum {  // a row's running (m, l, o)
@@ -1614,7 +1619,7 @@ static int paged_attn_launch(const CUtensorMap& tq, const CUtensorMap& tqf, cons
   // nothing to join where no item is long enough to be divided
   if (static_cast<long long>(p.width) << p.page_log2 <= stdb::PA_WHOLE * stdb::PA_BN)
     return cudaGetLastError() == cudaSuccess ? 0 : 4;
-  const dim3 mgrid(stdb::PA_CTAS, p.T > p.TQ ? 4 : 2);
+  const dim3 mgrid(stdb::PA_CTAS, p.T > p.TQ ? 4 : 2);  // (pairs are possible: two waves)
   if (launch_pdl(stdb::paged_merge_kernel<T, D>, mgrid, dim3(stdb::PM_THREADS), 0, s, p) != cudaSuccess) return 4;
   return cudaGetLastError() == cudaSuccess ? 0 : 4;
 }

@@ -91,3 +91,17 @@ def test_wrappers_refuse_cpu_tensors():
 @pytest.mark.parametrize("scale", [2.4e38, 3e38, 3.3e38])
 def test_attention_refuses_scales_that_overflow_in_log2(scale):
     assert attn(scale=scale) == 1
+
+
+@pytest.mark.parametrize("fits,over", [
+    (dict(T=2 ** 30 - 1, Hq=4), dict(T=2 ** 30, Hq=4)),
+    (dict(width=8388603, page=256), dict(width=8388604, page=256)),            # max_blocks * page_size <= 2^31 - 1025
+    (dict(pages=2 ** 21 - 2, page=256, Hkv=28), dict(pages=2 ** 22, page=256, Hkv=28)),
+    (dict(pages=2396744, page=256, Hkv=28), dict(pages=2396745, page=256, Hkv=28)),  # (num_pages + 1) * Hkv * page / 8 < 2^31
+])
+def test_attention_limits_are_those_of_the_header(fits, over):
+    """On the near side of each limit a call gets past the checks (and fails for want of
+    a device), on the far side it is refused."""
+    assert attn(**over) == 1
+    if not torch.cuda.is_available():
+        assert attn(**fits) not in (0, 1, 5)
