@@ -315,7 +315,8 @@ int std_collect_relevance(const void* q, const void* k_cache, const int32_t* vis
  * [0, max_blocks] refuses the request and is reported (device error 3), as are
  * more than max_tokens tokens unless max_tokens is 0 (the rest have no slot);
  * a page id or list length outside the pool is reported (error 2), the id gives
- * slot -1.  Inputs and outputs must not overlap. */
+ * slot -1.  A page is in one request's row or on the list, once.  What the call
+ * writes overlaps none of its other arrays (status 1). */
 int std_paged_update(const int32_t* past_lens, const int32_t* new_lens, int32_t* block_table, int32_t* n_blocks,
                      int32_t* free_pages, int32_t* n_free, int B, int max_blocks, int page_size, int num_pages,
                      int max_tokens, int32_t* cu_q, int32_t* kv_lens, int32_t* slots, int32_t* positions,
@@ -327,7 +328,8 @@ int std_paged_update(const int32_t* past_lens, const int32_t* new_lens, int32_t*
  * pools.  positions[t] < 0: row t is skipped, q_out's row left as it was;
  * slots[t] < 0: k and v are not stored.  A position >= max_pos is reported and
  * read as max_pos - 1, a slot outside the pool is reported and not stored
- * (error 2).  Slots of a call must differ. */
+ * (error 2).  Slots of a call must differ.  q_out and the pools overlap none of
+ * the call's other arrays (status 1), but for q_out = qkv with T 1. */
 int std_paged_rope_append(const void* qkv, int T, int Hq, int Hkv, int D, int is_fp16, const int32_t* positions,
                           const int32_t* slots, const void* cos_t, const void* sin_t, int max_pos, void* q_out,
                           void* k_pages, void* v_pages, int num_pages, int page_size, void* stream);
@@ -347,7 +349,8 @@ int std_paged_rope_append(const void* qkv, int T, int Hq, int Hkv, int D, int is
  * 3), the request skipped or its keys cut; a page id outside the pool is
  * reported (error 2) and read as zeros.
  * Same inputs, same bits; a request's last bits may depend on the batch it is
- * in (std_verify_attn's do not).  out and lse overlap no input.  The workspace
+ * in (std_verify_attn's do not).  out, lse and the workspace overlap none of the
+ * call's other arrays (status 1).  The workspace
  * (std_paged_attn_workspace_bytes, 32-byte aligned) is that of one call at a
  * time.
  * Limits beside the section's (status 1): T < 2^30, max_blocks * page_size <=

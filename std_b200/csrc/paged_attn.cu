@@ -1647,6 +1647,13 @@ extern "C" int std_paged_attn(const void* q, const void* k_pages, const void* v_
   if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 31) != 0 ||
       workspace_bytes < std_paged_attn_workspace_bytes(D))
     return 5;
+  const unsigned long long rows = static_cast<unsigned long long>(T) * Hq,
+                           pool = 2ull * D * Hkv * num_pages * page_size;
+  if (paged_overlap<9>({{q, rows * D * 2, false}, {k_pages, pool, false}, {v_pages, pool, false},
+                        {block_table, 4ull * B * max_blocks, false}, {cu_q, 4ull * B + 4, false},
+                        {kv_lens, 4ull * B, false}, {out, rows * D * 2, true}, {lse, lse == nullptr ? 0 : rows * 4, true},
+                        {workspace, std_paged_attn_workspace_bytes(D), true}}))
+    return 1;
   const int G = Hq / Hkv, TQ = 128 / G, TQ_few = stdb::PA_FEW / G;
   CUtensorMap tq, tqf, tk, tv;
   {

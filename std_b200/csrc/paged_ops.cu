@@ -332,6 +332,23 @@ __global__ void __launch_bounds__(512) paged_append_kernel(const PagedAppendPara
 static bool paged_page_ok(int page) { return page == 16 || page == 32 || page == 64 || page == 128 || page == 256; }
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// A call's arrays: true when one that it writes shares bytes with any other.
+struct PagedArray {
+  const void* p;
+  unsigned long long bytes;
+  bool written;
+};
+template <int N>
+static bool paged_overlap(const PagedArray (&a)[N]) {
+  for (int i = 0; i < N; ++i)
+    for (int j = 0; j < i; ++j) {
+      if ((!a[i].written && !a[j].written) || a[i].bytes == 0 || a[j].bytes == 0) continue;
+      const unsigned long long x = reinterpret_cast<uintptr_t>(a[i].p), y = reinterpret_cast<uintptr_t>(a[j].p);
+      if (x < y + a[j].bytes && y < x + a[i].bytes) return true;
+    }
+  return false;
+}
+
 extern "C" int std_paged_update(const int32_t* past_lens, const int32_t* new_lens, int32_t* block_table,
                                 int32_t* n_blocks, int32_t* free_pages, int32_t* n_free, int B, int max_blocks,
                                 int page_size, int num_pages, int max_tokens, int32_t* cu_q, int32_t* kv_lens,
@@ -348,6 +365,11 @@ extern "C" int std_paged_update(const int32_t* past_lens, const int32_t* new_len
       free_pages == nullptr || n_free == nullptr || cu_q == nullptr || kv_lens == nullptr || admitted == nullptr)
     return 1;
   if (max_tokens > 0 && (slots == nullptr || positions == nullptr)) return 1;
+  const unsigned long long n = 4ull * B, nt = 4ull * max_tokens;
+  if (paged_overlap<11>({{past_lens, n, false}, {new_lens, n, false}, {block_table, n * max_blocks, true},
+                         {n_blocks, n, true}, {free_pages, 4ull * num_pages, true}, {n_free, 4, true}, {cu_q, n + 4, true},
+                         {kv_lens, n, true}, {slots, nt, true}, {positions, nt, true}, {admitted, n, true}}))
+    return 1;
   stdb::PagedUpdateParams p;
   p.past = past_lens;
   p.fresh = new_lens;
@@ -396,6 +418,12 @@ extern "C" int std_paged_rope_append(const void* qkv, int T, int Hq, int Hkv, in
     return 1;
   if (!aligned16(qkv) || !aligned16(cos_t) || !aligned16(sin_t) || !aligned16(q_out) || !aligned16(k_pages) ||
       !aligned16(v_pages))
+    return 1;
+  const unsigned long long row = 2ull * D, pool = row * Hkv * num_pages * page_size;
+  const bool in_place = T == 1 && q_out == qkv;  // (a thread writes what it has read)
+  if (paged_overlap<8>({{qkv, in_place ? 0 : row * T * (Hq + 2 * Hkv), false}, {positions, 4ull * T, false},
+                        {slots, 4ull * T, false}, {cos_t, row / 2 * max_pos, false}, {sin_t, row / 2 * max_pos, false},
+                        {q_out, row * T * Hq, true}, {k_pages, pool, true}, {v_pages, pool, true}}))
     return 1;
   stdb::PagedAppendParams p;
   p.qkv = qkv;

@@ -451,7 +451,8 @@ def paged_update(past_lens: torch.Tensor, new_lens: torch.Tensor, block_table: t
     shorter past_lens rolls a request back.  Returns (cu_q [B + 1], kv_lens [B],
     slots [max_tokens], positions [max_tokens], admitted [B]); a request that the
     list cannot serve has admitted 0, kv_lens 0 and slots -1.  A step without
-    requests (B 0) gives cu_q [0] and slots of -1.  `out` gives the
+    requests (B 0) gives cu_q [0] and slots of -1.  What the call writes shares no
+    memory with its other tensors (status 1).  `out` gives the
     five result tensors (a captured graph's static buffers; the captured body of a
     loop or branch needs it)."""
     device = _paged_device(past_lens, "past_lens")
@@ -497,7 +498,8 @@ def paged_rope_append(qkv: torch.Tensor, positions: torch.Tensor, slots: torch.T
     """RoPE of qkv [T, (Hq + 2 Hkv) * D]'s q and k at positions [T]; q goes to
     q_out [T, Hq, D], k and v to slots [T] of the pools [num_pages, Hkv, page,
     D].  Position -1: the row is skipped; slot -1: nothing is stored.  bf16 or
-    fp16 throughout (tables cos_t, sin_t [max_pos, D / 2] too)."""
+    fp16 throughout (tables cos_t, sin_t [max_pos, D / 2] too).  q_out and the pools
+    share no memory with the call's other tensors (status 1)."""
     device = _paged_device(qkv, "qkv")
     dtype = qkv.dtype
     if dtype not in _PAGED_DTYPES:
@@ -543,7 +545,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     1] int32); pools [num_pages, Hkv, page, D]; block_table [B, max_blocks] and
     kv_lens [B] int32, the new tokens' keys included.  Token t of n sees keys 0 ..
     kv_len - n + t (causal) or all kv_len.  bf16 or fp16; any Hq / Hkv up to 128.
-    scale defaults to 1 / sqrt(D).  out [T, Hq, D], lse [T, Hq] fp32 (optional).
+    scale defaults to 1 / sqrt(D).  out [T, Hq, D], lse [T, Hq] fp32 (optional),
+    which share no memory with the call's other tensors (status 1).
     Rows that see no key give 0 and -inf; rows outside every request are left
     as they were (uninitialised in an `out` made here): all of them in a step
     without requests.  workspace (optional): a

@@ -102,6 +102,59 @@ def test_attention_refuses_scales_that_overflow_in_log2(scale):
 def test_attention_limits_are_those_of_the_header(fits, over):
     """On the near side of each limit a call gets past the checks (and fails for want of
     a device), on the far side it is refused."""
-    assert attn(**over) == 1
+    apart = dict(zip(("q", "k", "v", "table", "cu", "lens", "out", "ws"), range(1 << 44, 9 << 44, 1 << 44)))
+    assert attn(**apart, **over) == 1
     if not torch.cuda.is_available():
-        assert attn(**fits) not in (0, 1, 5)
+        assert attn(**apart, **fits) not in (0, 1, 5)
+
+
+# Arrays of a call, each at an address of its own (never read: without a device no call gets that far).
+def apart(*names):
+    return {n: (i + 1) << 44 for i, n in enumerate(names)}
+
+
+UPDATE = apart("past", "new", "table", "nblk", "free", "nfree", "cu", "kv", "slots", "pos", "ok")
+APPEND = apart("qkv", "pos", "slots", "cos", "sin", "q", "k", "v")
+ATTN = apart("q", "k", "v", "table", "cu", "lens", "out", "lse", "ws")
+SIZES = {  # bytes of each, for the sizes that update(), append() and attn() give
+    "update": dict(past=8, new=8, table=32, nblk=8, free=32, nfree=4, cu=12, kv=8, slots=12, pos=12, ok=8),
+    "append": dict(qkv=3 * 36 * 256, pos=12, slots=12, cos=9 * 128, sin=9 * 128, q=3 * 28 * 256, k=8 * 4 * 16 * 256,
+                   v=8 * 4 * 16 * 256),
+    "attn": dict(q=4 * 28 * 256, k=8 * 4 * 16 * 256, v=8 * 4 * 16 * 256, table=16, cu=8, lens=4, out=4 * 28 * 256,
+                 lse=4 * 28 * 4, ws=2 * 148 * 256 * (128 * 4 + 8)),
+}
+CALLS = {"update": (update, UPDATE, {"past", "new"}), "append": (append, APPEND, {"qkv", "pos", "slots", "cos", "sin"}),
+         "attn": (attn, ATTN, {"q", "k", "v", "table", "cu", "lens"})}
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: only where no call can launch")
+@pytest.mark.parametrize("name", CALLS)
+def test_overlapping_arrays_are_refused(name):
+    call, at, read = CALLS[name]
+    assert call(**at) in (3, 4)  # past the checks: no device here
+    for a in at:
+        for b in at:
+            if a == b:
+                continue
+            for shift in (0, SIZES[name][b] - 1 & ~31):  # b's first bytes, and its last ones
+                got = call(**{**at, a: at[b] + shift})
+                assert got == 1 if not {a, b} <= read else got in (3, 4), (a, b, shift)
+            if b != "ws":  # right behind b
+                assert call(**{**at, a: at[b] + (SIZES[name][b] + 31 & ~31)}) in (3, 4), (a, b)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: only where no call can launch")
+def test_one_row_may_be_rotated_in_place():
+    assert append(**{**APPEND, "q": APPEND["qkv"], "T": 1}) in (3, 4)
+    assert append(**{**APPEND, "q": APPEND["qkv"] + 256, "T": 1}) == 1
+
+
+@pytest.mark.parametrize("call,args,bad", [
+    (update, UPDATE, dict(B=0)), (update, UPDATE, dict(page=24)), (update, UPDATE, dict(tokens=-1)),
+    (update, UPDATE, dict(table=None)), (update, UPDATE, dict(slots=None)), (update, UPDATE, dict(pages=1 << 28)),
+    (append, APPEND, dict(D=80)), (append, APPEND, dict(max_pos=0)), (append, APPEND, dict(q=None)),
+    (append, APPEND, dict(qkv=APPEND["qkv"] + 2)), (append, APPEND, dict(pages=1 << 28)),
+    (attn, ATTN, dict(D=96)), (attn, ATTN, dict(scale=0.0)), (attn, ATTN, dict(out=ATTN["out"] + 4)),
+    (attn, ATTN, dict(Hq=30)), (attn, ATTN, dict(page=48)), (attn, ATTN, dict(cu=None))])
+def test_refusals_with_arrays_apart(call, args, bad):
+    assert call(**{**args, **bad}) == 1

@@ -395,6 +395,41 @@ def test_steps_without_requests(ops, graph):
     _no_device_error(ops)
 
 
+def test_results_over_inputs_are_refused(ops):
+    """Lengths advanced in place would lose a refused request's, q over qkv would race, out over
+    a workspace or a pool too: refused, nothing changed.  One row may be rotated in place."""
+    past, new, held, n_free = _i32([3, 0]), _i32([20, 3]), _i32([0, 0]), _i32([8])
+    table, free = torch.full((2, 8), -1, dtype=torch.int32, device="cuda"), torch.arange(8, device="cuda").int()
+    e = lambda n: torch.empty(n, dtype=torch.int32, device="cuda")  # noqa: E731
+    for out in ((e(3), past, e(23), e(23), e(2)), (e(3), e(2), e(23), e(23), new), (e(3), held, e(23), e(23), e(2))):
+        with pytest.raises(RuntimeError, match="status 1"):
+            ops.paged_update(past, new, table, held, free, n_free, 16, 23, out=out)
+    assert past.tolist() == [3, 0] and new.tolist() == [20, 3] and held.tolist() == [0, 0] and n_free.item() == 8
+    cos = torch.ones(4, 64, dtype=BF, device="cuda")
+    k = torch.zeros(5, 4, 16, 128, dtype=BF, device="cuda")
+    v = torch.zeros_like(k)
+    qkv = torch.randn(3, 36 * 128, device="cuda").to(BF)
+    before, i = qkv.clone(), _i32([0, 1, 2])
+    with pytest.raises(RuntimeError, match="status 1"):
+        ops.paged_rope_append(qkv, i, i, cos, cos, qkv.view(-1)[:3 * 28 * 128].view(3, 28, 128), k, v)
+    with pytest.raises(RuntimeError, match="status 1"):
+        ops.paged_rope_append(qkv, i, i, cos, cos, torch.empty(3, 28, 128, dtype=BF, device="cuda"), k, k)
+    assert torch.equal(qkv, before) and (k == 0).all()
+    one, sin = qkv[:1].clone(), torch.full_like(cos, 0.5)
+    apart = ops.paged_rope_append(one, i[1:2], i[1:2], cos, sin, torch.empty(1, 28, 128, dtype=BF, device="cuda"), k, v)
+    ops.paged_rope_append(one, i[1:2], i[1:2], cos, sin, one[:, :28 * 128].view(1, 28, 128), k, v)
+    assert torch.equal(one[:, :28 * 128].view(1, 28, 128), apart)
+    x = Paged([(30, 2)], 28, 4, 128, 16, BF)
+    ws = ops.paged_attention_workspace(128)
+    with pytest.raises(RuntimeError, match="status 1"):
+        x.call(ops, workspace=ws, out=ws[:x.q.numel() * 2].view(BF).view(x.q.shape))
+    with pytest.raises(RuntimeError, match="status 1"):
+        x.call(ops, out=x.k.view(-1)[:x.q.numel()].view(x.q.shape))
+    with pytest.raises(RuntimeError, match="status 1"):
+        x.call(ops, lse=x.q.view(-1)[:x.q.shape[0] * 28 * 2].view(torch.float32).view(-1, 28))
+    _no_device_error(ops)
+
+
 # ------------------------------------------------------------------ long prompts
 def test_long_prompt_every_row_against_64_bits(ops):
     """A 40,000-token prompt at once and in odd chunks: every row within its own rounding of
