@@ -48,9 +48,9 @@
 // query heads on 4 key heads, D 128 unless said).  Long prompts: the softmax warps
 // and power; a 2048-token chunk over 31K keys 825 us = 1130 TFLOP/s in a short run
 // (0.69 of cuBLAS's burst; 3200 cycles a block of a pair, of which a softmax warp
-// works 2900 and the MMAs need 2560; 1.45 GHz) and 945 us = 990 TFLOP/s in a long one
-// (0.72 of what cuBLAS sustains under the power cap; 1.3 GHz), an 8192-token prompt
-// 508 and 528 us.  S in halves costs 1.5 x the shared-memory reads of N=128 but keeps
+// works 2900 and the MMAs need 2560; 1.45 GHz) and 924 to 945 us = 990 to 1010 TFLOP/s
+// in a long one (0.72 to 0.74 of what cuBLAS sustains under the power cap; 1.3 GHz), an
+// 8192-token prompt 508 and 518 to 528 us.  S in halves costs 1.5 x the shared-memory reads of N=128 but keeps
 // a half of S ready while the other is multiplied: 866 us with one S of 128 columns a
 // step from one issuing thread, 815 with halves and a thread per stream (at the same
 // clock, before the sums of O were divided).
@@ -510,12 +510,15 @@ STD_DEV bool paged_softmax_half(uint32_t tS, uint32_t tO, float sc, int nvis, bo
   for (int j = 8; j < N; j += 8)
 #pragma unroll
     for (int c = 0; c < 4; ++c) m4[c] = max3(m4[c], __uint_as_float(x[j + c]), __uint_as_float(x[j + 4 + c]));
-  const float m_c = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * sc;  // scale > 0
-  const bool need = m_run != -INFINITY && m_c > m_run + (PA_RESCALE + PA_TOP<T>);
+  const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+  const float m_c = fmaf(mx, sc, -PA_TOP<T>);  // scale > 0
+  // (the exponent that P gets, not a difference of rounded ones: at 2^24 those are off by
+  // 2, and a half would overflow)
+  const bool need = m_run != -INFINITY && fmaf(mx, sc, -m_run) > PA_RESCALE + PA_TOP<T>;
   if (__any_sync(0xffffffffu, need)) {
     if (!__all_sync(0xffffffffu, mbar_wait(bar_next, next & 1))) return false;  // O at rest
     tc_fence_after();
-    const float alpha = need ? exp2f(m_run - (m_c - PA_TOP<T>)) : 1.0f;
+    const float alpha = need ? exp2f(m_run - m_c) : 1.0f;
     uint32_t o[32];
 #pragma unroll 1
     for (int c = 0; c < D / 32; ++c) {
@@ -527,10 +530,10 @@ STD_DEV bool paged_softmax_half(uint32_t tS, uint32_t tO, float sc, int nvis, bo
     }
     if (need) {
       l_run *= alpha;
-      m_run = m_c - PA_TOP<T>;
+      m_run = m_c;
     }
   }
-  if (m_run == -INFINITY) m_run = m_c - PA_TOP<T>;
+  if (m_run == -INFINITY) m_run = m_c;
   // a row that has seen no key yet keeps P = 2^-inf = 0
   const float nm = m_run == -INFINITY ? 0.f : -m_run;
   const uint64_t sc2 = f2_make(sc, sc), nm2 = f2_make(nm, nm);

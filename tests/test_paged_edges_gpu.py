@@ -286,6 +286,39 @@ def test_many_small_weights_beside_a_large_one(ops, new, D, dtype, below):
     _no_device_error(ops)
 
 
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("log2", [16, 20, 22, 23, 24, 25, 26, 27])
+def test_scores_of_great_size(ops, dtype, log2):
+    """Scores of 2^16 to 2^27, which 32 bits hold to 2^-8 to 8, with differences on both sides
+    of what raises a maximum.  Their rounding decides the weights, so what holds is that
+    each output is a mean of the values: between their least and greatest, but for the
+    roundings of output and probabilities (e / 2 each, of one sign here) and the sums."""
+    D, e = 128, torch.finfo(dtype).eps
+    for step in (0.0, 4.0, 9.0, 14.0, 30.0):
+        x = Paged([(700, 1), (690, 4), (2000, 15), (600, 100)], 14, 2, D, 64, dtype, seed=log2)
+        big = 2 ** (log2 / 2) * math.sqrt(math.log(2) * math.sqrt(D))
+        x.q = torch.zeros_like(x.q)
+        x.q[..., 0], x.q[..., 1] = big, math.sqrt(D)
+        x.keys = [(k, v.abs() + 0.5) for k, v in x.keys]
+        x.v = x.v.abs() + 0.5
+        for b in range(len(x.pairs)):
+            keys, L = torch.zeros_like(x.keys[b][0]), x.kv[b]
+            keys[..., 0] = big
+            jump = torch.arange(L, device="cuda") // 64 % 5 * step
+            keys[..., 1] = ((jump[:, None] + x.keys[b][0][..., 1].float()) * math.log(2)).to(dtype)
+            set_keys(x, b, keys)
+        lse = torch.empty(x.q.shape[:2], device="cuda")
+        out, at = x.call(ops, lse=lse).double(), 0
+        assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+        for b, (_, n) in enumerate(x.pairs):
+            v = x.keys[b][1].double().repeat_interleave(7, 1)
+            lo, hi = v.amin(0), v.amax(0)
+            slack = 1.01 * (e + 2.0 ** -12)
+            assert (out[at:at + n] >= lo * (1 - slack)).all() and (out[at:at + n] <= hi * (1 + slack)).all(), (b, step)
+            at += n
+    _no_device_error(ops)
+
+
 # ------------------------------------------------------------------ idle requests
 @pytest.mark.parametrize("B", [33, 64, 2047, 8192])
 def test_mostly_idle_batches(ops, B):
