@@ -72,10 +72,10 @@ constexpr int PA_CTAS = 148;     // one CTA per SM
 constexpr int PA_THREADS = 384;  // 2 softmax warpgroups; TMA, two MMA and a scheduler warp
 constexpr int PA_BN = 128;       // keys per block
 constexpr float PA_RESCALE = 8.0f;  // log2 units
-// log2 of the largest P when m is set: P lies between 2^-24 (a half's smallest
-// number) and 2^(top + PA_RESCALE) at most, below a half's 65504.  Weights under 2^(-25 - top) of the
-// largest are lost, which many keys of small weight beside a heavy one notice (2^17
-// keys of 2^-25 each: 0.4 % of the row with top 0).  bf16 has the range of a float.
+// m is set this far below the maximum, in log2 units: P is 2^top there and stays below
+// 2^(top + PA_RESCALE), for fp16 below its 65504.  Weights under 2^(-25 - top) of the
+// largest are lost in fp16, which many keys of small weight beside a heavy one notice
+// (2^17 keys of 2^-25 each: 0.4 % of the row with top 0).  bf16 has the range of a float.
 template <typename T>
 constexpr float PA_TOP = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 // Cost of a block in a single and in a pair (measured: 2000 to 2400 cycles and
@@ -209,7 +209,7 @@ struct PagedWalk {
   }
   // On to the next request with tokens, 32 at a time, a request per lane (a batch
   // of fixed size may be idle for the most part: 8192 requests, two at each end with
-  // tokens: 1587 us when they were passed one by one).  False: there is none.
+  // tokens: 231 us, and 1583 when they were passed one by one).  False: there is none.
   STD_DEV bool next_request(const PagedAttnParams& p) {
     const int lane = threadIdx.x & 31;
     for (++b; b < p.B; b += 32) {
@@ -592,10 +592,10 @@ STD_DEV int warp_reduce_rows(float* v, int lane, Op op) {
 // stream's S, O, join and group barriers; bar_q_empty: its query slot's.  False
 // when a wait ran out.  sV: the stage of the piece's last V; ntail: tails cleared.
 //
-// m (sh.ref) is set to the row's maximum over the first block that has one (a
-// visible score above -inf: as a rule the first block) and raised when a score passes
-// it by 2^8, on all four warps: they vote at every block.  Until it is set it is 0, the
-// row's P, l and O are 0, and the vote is taken as given.
+// m (sh.ref) is set by the row's maximum over the first block that has one (a
+// visible score above -inf: as a rule the first block) and raised when a P would pass
+// 2^(PA_RESCALE + PA_TOP), on all four warps: they vote at every block.  Until it is set
+// it is 0, the row's P, l and O are 0, and the vote is taken as given.
 template <typename T, int D, int N, int ST>
 STD_DEV bool paged_few_piece(const PagedAttnParams& p, const PagedPiece& piece, PagedShared<ST>& sh, uint8_t* sQ,
                              uint8_t* sV, uint32_t tS, uint32_t tO, int s, uint64_t* bar_q_empty, uint32_t& ntail,
